@@ -406,7 +406,6 @@ def _own(s):
         s["adamw"].step(s["grads"], lr=LR)
         out = {k: s[k] for k in ("param", "copy") if k in s}
         out.update(s["adamw"].state())
-        out.pop("steps")
         return out
     if kind == "priors":
         return learner.priors(s["logits"], legal=s["legal"])
