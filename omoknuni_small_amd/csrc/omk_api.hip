@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "omk_internal.h"
+#include "omk_learn_internal.h"
 #include "omk_priors.h"
 #include "omk_staging.h"
 
@@ -24,6 +25,15 @@ using namespace omk;
 static thread_local char g_err[512] = "";
 
 static int fail(int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+// The same for the operators of include/omk_learn.h: one message per thread, whichever call failed.
+int omk::learn_fail(int code, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);

@@ -1,0 +1,480 @@
+// C ABI of include/omk_learn.h: handles, checks of arguments, and the launches.
+#include "../../include/omk_learn.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <exception>
+#include <new>
+#include <vector>
+
+#include "omk_learn_internal.h"
+
+using namespace omk;
+
+struct omk_learner {
+    int device = 0;
+    hipStream_t stream = nullptr;
+    int children = 0;       // optimizers that live
+    bool released = false;  // omk_learner_destroy was called while some did
+};
+
+struct omk_adamw {
+    omk_learner *l = nullptr;
+    int32_t n_tensors = 0;
+    int32_t param_type = 0, grad_type = 0, copy_type = 0, state_type = 0;
+    double beta1 = 0, beta2 = 0, eps = 0;
+    uint32_t seed = 0;
+    char *memory = nullptr;  // the count, the tensors, the chunks
+    AdamCount *count = nullptr;
+    AdamTensor *tensors = nullptr;
+    AdamChunk *chunks = nullptr;
+    std::vector<int64_t> first_chunk;  // of every tensor, and the end
+    std::vector<int64_t> elements;
+};
+
+namespace {
+
+// The calling thread's device is the learner's while one of these lives.
+struct OnDevice {
+    int before = -1;
+    hipError_t status;
+    explicit OnDevice(int device) {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && before != device) status = hipSetDevice(device);
+        if (status == hipSuccess && before == device) before = -1;
+        (void)hipGetLastError();  // launches are checked with hipGetLastError: start from a clean slate
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+#define LEARN_TRY(expr)                                                                                \
+    do {                                                                                               \
+        hipError_t e_ = (expr);                                                                        \
+        if (e_ != hipSuccess) return learn_fail(OMK_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+    } while (0)
+
+// No C++ exception crosses the C boundary.
+#define LEARN_NO_THROW \
+    catch (const std::exception &e_) { return learn_fail(OMK_ERR_INVALID, "out of host memory (%s)", e_.what()); }
+
+int width_of(int type) { return type == OMK_F32 ? 4 : type == OMK_F8 ? 1 : 2; }
+bool float_type(int type) { return type == OMK_F32 || type == OMK_BF16 || type == OMK_F16; }
+bool aligned(const void *p, int width) { return ((uintptr_t)p & (uintptr_t)(width - 1)) == 0; }
+
+// Bytes from the first element of a matrix to behind its last; -1 where that passes 62 bits.
+int64_t span_bytes(int64_t rows, int64_t stride, int64_t columns, int width) {
+    const __int128 n = ((__int128)(rows - 1) * stride + columns) * width;
+    return n >> 62 ? -1 : (int64_t)n;
+}
+
+bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
+int check_rows(const char *who, const omk_policy_rows *r, Rows *out) {
+    if (!float_type(r->type)) return learn_fail(OMK_ERR_INVALID, "%s: logits of type %d", who, r->type);
+    if (r->rows < 0 || r->rows > INT32_MAX)
+        return learn_fail(OMK_ERR_INVALID, "%s: %lld rows", who, (long long)r->rows);
+    if (r->actions < 1 || r->actions > OMK_MAX_ACTIONS)
+        return learn_fail(OMK_ERR_INVALID, "%s: %d actions (1 .. %d)", who, r->actions, OMK_MAX_ACTIONS);
+    const int words = (r->actions + 31) / 32;
+    if (r->rows > 1 && r->row_stride < r->actions)
+        return learn_fail(OMK_ERR_INVALID, "%s: rows of %d actions, %lld apart", who, r->actions, (long long)r->row_stride);
+    if (r->d_legal && (r->legal_stride < 0 || (r->rows > 1 && r->legal_stride && r->legal_stride < words)))
+        return learn_fail(OMK_ERR_INVALID, "%s: masks of %d words, %lld apart", who, words, (long long)r->legal_stride);
+    if (r->rows && !r->d_logits) return learn_fail(OMK_ERR_INVALID, "%s: no logits", who);
+    if (!aligned(r->d_logits, width_of(r->type)) || !aligned(r->d_legal, 4))
+        return learn_fail(OMK_ERR_INVALID, "%s: an address that is no multiple of its type's size", who);
+    if (r->rows && (span_bytes(r->rows, r->row_stride, r->actions, width_of(r->type)) < 0 ||
+                    (r->d_legal && span_bytes(r->rows, r->legal_stride, words, 4) < 0)))
+        return learn_fail(OMK_ERR_INVALID, "%s: rows that pass the address space", who);
+    *out = Rows{r->d_logits, r->row_stride, r->rows, r->actions, r->d_legal, r->legal_stride};
+    return OMK_OK;
+}
+
+// A matrix of results beside the logits: apart from them, or (in_place) just where they are.
+int check_result(const char *who, const char *what, const omk_policy_rows *r, const void *d, int64_t stride, int width,
+                 bool in_place) {
+    if (!d) return learn_fail(OMK_ERR_INVALID, "%s: no %s", who, what);
+    if (!aligned(d, width)) return learn_fail(OMK_ERR_INVALID, "%s: %s at an address that is no multiple of its type's size", who, what);
+    if (r->rows > 1 && stride < r->actions)
+        return learn_fail(OMK_ERR_INVALID, "%s: %s rows of %d actions, %lld apart", who, what, r->actions, (long long)stride);
+    const int64_t bytes = span_bytes(r->rows, stride, r->actions, width);
+    if (bytes < 0) return learn_fail(OMK_ERR_INVALID, "%s: rows that pass the address space", who);
+    const int64_t of_logits = span_bytes(r->rows, r->row_stride, r->actions, width_of(r->type));
+    if (in_place && d == r->d_logits && (r->rows < 2 || stride == r->row_stride)) return OMK_OK;
+    if (overlap(d, bytes, r->d_logits, of_logits))
+        return learn_fail(OMK_ERR_INVALID, "%s: the %s lies across the logits", who, what);
+    return OMK_OK;
+}
+
+bool aligned4(const char *who, const void *const *p, int n) {
+    for (int i = 0; i < n; i++)
+        if (!aligned(p[i], 4)) {
+            learn_fail(OMK_ERR_INVALID, "%s: an address that is no multiple of its type's size", who);
+            return false;
+        }
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int omk_learner_create(int32_t device, omk_learner **out) {
+    if (!out) return learn_fail(OMK_ERR_INVALID, "omk_learner_create: null argument");
+    int count = 0;
+    LEARN_TRY(hipGetDeviceCount(&count));
+    if (device < 0 || device >= count)
+        return learn_fail(OMK_ERR_INVALID, "omk_learner_create: device %d of %d", device, count);
+    omk_learner *l = new (std::nothrow) omk_learner();
+    if (!l) return learn_fail(OMK_ERR_INVALID, "out of host memory");
+    l->device = device;
+    *out = l;
+    return OMK_OK;
+}
+
+int omk_learner_destroy(omk_learner *l) {
+    if (l && l->children)
+        l->released = true;  // goes with the last of its optimizers
+    else
+        delete l;
+    return OMK_OK;
+}
+
+int omk_learner_set_stream(omk_learner *l, void *hip_stream) {
+    if (!l) return learn_fail(OMK_ERR_INVALID, "omk_learner_set_stream: null argument");
+    l->stream = (hipStream_t)hip_stream;
+    return OMK_OK;
+}
+
+int omk_learner_get_stream(omk_learner *l, void **hip_stream_out) {
+    if (!l || !hip_stream_out) return learn_fail(OMK_ERR_INVALID, "omk_learner_get_stream: null argument");
+    *hip_stream_out = (void *)l->stream;
+    return OMK_OK;
+}
+
+int omk_learner_sync(omk_learner *l) {
+    if (!l) return learn_fail(OMK_ERR_INVALID, "omk_learner_sync: null argument");
+    OnDevice on(l->device);
+    LEARN_TRY(on.status);
+    LEARN_TRY(hipStreamSynchronize(l->stream));
+    return OMK_OK;
+}
+
+int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride) {
+    const char *who = "omk_policy_priors";
+    if (!l || !rows) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    Rows r;
+    if (int rc = check_rows(who, rows, &r)) return rc;
+    if (!r.rows) return OMK_OK;
+    if (int rc = check_result(who, "priors", rows, d_priors, prior_stride, 4, false)) return rc;
+    OnDevice on(l->device);
+    LEARN_TRY(on.status);
+    LEARN_TRY(launch_priors(rows->type, r, d_priors, prior_stride, l->stream));
+    return OMK_OK;
+}
+
+int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32_t *d_moves, float *d_logprob,
+                        float *d_entropy) {
+    const char *who = "omk_policy_logprobs";
+    if (!l || !rows) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    Rows r;
+    if (int rc = check_rows(who, rows, &r)) return rc;
+    if (d_logprob && !d_moves && r.rows) return learn_fail(OMK_ERR_INVALID, "%s: no moves", who);
+    const void *all[] = {d_moves, d_logprob, d_entropy};
+    if (!aligned4(who, all, 3)) return OMK_ERR_INVALID;
+    if (!r.rows || (!d_logprob && !d_entropy)) return OMK_OK;
+    OnDevice on(l->device);
+    LEARN_TRY(on.status);
+    LEARN_TRY(launch_logprobs(rows->type, r, d_moves, d_logprob, d_entropy, l->stream));
+    return OMK_OK;
+}
+
+int64_t omk_policy_loss_work(int64_t rows, int32_t actions) {
+    (void)actions;
+    return rows > 0 ? rows * 4 : 0;
+}
+
+int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_policy_samples *samples,
+                    const omk_policy_loss_params *params, const omk_policy_loss_out *out, void *d_work,
+                    int64_t work_bytes) {
+    const char *who = "omk_policy_loss";
+    if (!l || !rows || !samples || !params || !out) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    Rows r;
+    if (int rc = check_rows(who, rows, &r)) return rc;
+    if (!(params->clip_low >= 0.0) || !(params->clip_high >= 0.0) || !std::isfinite(params->clip_high))
+        return learn_fail(OMK_ERR_INVALID, "%s: clipped to [1 - %g, 1 + %g]", who, params->clip_low, params->clip_high);
+    if (!(params->kl_weight >= 0.0) || !std::isfinite(params->kl_weight) || !std::isfinite(params->scale))
+        return learn_fail(OMK_ERR_INVALID, "%s: kl_weight %g, scale %g", who, params->kl_weight, params->scale);
+    if (params->kl_weight > 0.0 && !samples->d_ref_logprob)
+        return learn_fail(OMK_ERR_INVALID, "%s: a KL term needs the reference's log-probabilities", who);
+    if (!out->d_loss) return learn_fail(OMK_ERR_INVALID, "%s: no loss", who);
+    const void *all[] = {samples->d_moves, samples->d_old_logprob, samples->d_advantage, samples->d_ref_logprob,
+                         samples->d_weight, out->d_loss, out->d_logprob, out->d_kl, d_work};
+    if (!aligned4(who, all, 9)) return OMK_ERR_INVALID;
+    if (r.rows) {
+        if (!samples->d_moves || !samples->d_old_logprob || !samples->d_advantage || !out->d_logprob)
+            return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+        if (out->d_grad)
+            if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
+                return rc;
+        const int64_t needed = omk_policy_loss_work(r.rows, r.actions);
+        if (needed && (!d_work || work_bytes < needed))
+            return learn_fail(OMK_ERR_CAPACITY, "%s: %lld bytes of work space, %lld needed", who,
+                              (long long)(d_work ? work_bytes : 0), (long long)needed);
+    }
+    OnDevice on(l->device);
+    LEARN_TRY(on.status);
+    if (!r.rows) {
+        LEARN_TRY(launch_set_float(out->d_loss, 0.0f, l->stream));
+        return OMK_OK;
+    }
+    PolicyLoss p;
+    p.moves = samples->d_moves;
+    p.old_logprob = samples->d_old_logprob;
+    p.advantage = samples->d_advantage;
+    p.ref_logprob = samples->d_ref_logprob;
+    p.weight = samples->d_weight;
+    p.log_low = params->clip_low < 1.0 ? std::log(1.0 - params->clip_low) : -INFINITY;
+    p.log_high = std::log(1.0 + params->clip_high);
+    p.low = (float)(1.0 - params->clip_low);
+    p.high = (float)(1.0 + params->clip_high);
+    p.kl_weight = (float)params->kl_weight;
+    p.scale = (float)params->scale;
+    p.grad = out->d_grad;
+    p.grad_stride = out->grad_stride;
+    p.logprob = out->d_logprob;
+    p.kl = out->d_kl;
+    p.row_loss = (float *)d_work;
+    p.loss = out->d_loss;
+    LEARN_TRY(launch_policy_loss(rows->type, r, p, l->stream));
+    return OMK_OK;
+}
+
+int64_t omk_preference_loss_work(int64_t rows, int32_t actions, int64_t pairs) {
+    (void)actions;
+    return (rows > 0 ? rows * 16 : 0) + (pairs > 0 ? pairs * 4 : 0);
+}
+
+int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32_t *d_moves,
+                        const int32_t *d_line_begin, int64_t pairs, const float *d_ref_logprob,
+                        const omk_preference_params *params, const omk_preference_out *out, void *d_work,
+                        int64_t work_bytes) {
+    const char *who = "omk_preference_loss";
+    if (!l || !rows || !params || !out) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    Rows r;
+    if (int rc = check_rows(who, rows, &r)) return rc;
+    if (pairs < 0 || pairs > INT32_MAX / 2) return learn_fail(OMK_ERR_INVALID, "%s: %lld pairs", who, (long long)pairs);
+    if (!std::isfinite(params->beta) || !std::isfinite(params->scale) || !(params->label_smoothing >= 0.0) ||
+        !(params->label_smoothing <= 0.5))
+        return learn_fail(OMK_ERR_INVALID, "%s: beta %g, label_smoothing %g (0 .. 0.5), scale %g", who, params->beta,
+                          params->label_smoothing, params->scale);
+    if (!out->d_loss) return learn_fail(OMK_ERR_INVALID, "%s: no loss", who);
+    const void *all[] = {d_moves, d_line_begin, d_ref_logprob, out->d_loss, out->d_margin, out->d_line_logprob, d_work};
+    if (!aligned4(who, all, 7)) return OMK_ERR_INVALID;
+    if (pairs) {
+        if (!d_line_begin || (r.rows && !d_moves)) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+        if (r.rows && out->d_grad)
+            if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
+                return rc;
+        const int64_t needed = omk_preference_loss_work(r.rows, r.actions, pairs);
+        if (!d_work || work_bytes < needed)
+            return learn_fail(OMK_ERR_CAPACITY, "%s: %lld bytes of work space, %lld needed", who,
+                              (long long)(d_work ? work_bytes : 0), (long long)needed);
+    }
+    OnDevice on(l->device);
+    LEARN_TRY(on.status);
+    if (!pairs) {
+        LEARN_TRY(launch_set_float(out->d_loss, 0.0f, l->stream));
+        return OMK_OK;
+    }
+    PreferenceLoss p;
+    p.moves = d_moves;
+    p.line_begin = d_line_begin;
+    p.pairs = pairs;
+    p.ref_logprob = d_ref_logprob;
+    p.beta = (float)params->beta;
+    p.smoothing = (float)params->label_smoothing;
+    p.scale = (float)params->scale;
+    p.grad = r.rows ? out->d_grad : nullptr;
+    p.grad_stride = out->grad_stride;
+    p.zero_rest = out->zero_rest;
+    p.margin = out->d_margin;
+    p.line_logprob = out->d_line_logprob;
+    p.loss = out->d_loss;
+    float *work = (float *)d_work;
+    p.top = work;
+    p.inverse = work + r.rows;
+    p.logprob = work + 2 * r.rows;
+    p.slope = work + 3 * r.rows;
+    p.pair_loss = work + 4 * r.rows;
+    LEARN_TRY(launch_preference_loss(rows->type, r, p, l->stream));
+    return OMK_OK;
+}
+
+int omk_adamw_destroy(omk_adamw *o) {
+    if (!o) return OMK_OK;
+    {
+        OnDevice on(o->l->device);
+        if (o->memory) (void)hipFree(o->memory);  // (waits for the device)
+        (void)hipGetLastError();
+    }
+    if (--o->l->children == 0 && o->l->released) delete o->l;
+    delete o;
+    return OMK_OK;
+}
+
+int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out) try {
+    const char *who = "omk_adamw_create";
+    if (!l || !desc || !out || (desc->n_tensors > 0 && !desc->h_tensors))
+        return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    if (desc->n_tensors < 0 || desc->n_tensors > 1 << 24)
+        return learn_fail(OMK_ERR_INVALID, "%s: %d tensors", who, desc->n_tensors);
+    const int pt = desc->param_type, gt = desc->grad_type, ct = desc->copy_type, st = desc->state_type;
+    if (!float_type(pt)) return learn_fail(OMK_ERR_INVALID, "%s: parameters of type %d", who, pt);
+    if (!float_type(gt)) return learn_fail(OMK_ERR_INVALID, "%s: gradients of type %d", who, gt);
+    if (ct != OMK_NONE && ct != OMK_BF16 && ct != OMK_F16)
+        return learn_fail(OMK_ERR_INVALID, "%s: copies of type %d", who, ct);
+    if (st != OMK_F32 && st != OMK_F8) return learn_fail(OMK_ERR_INVALID, "%s: states of type %d", who, st);
+    if (pt != OMK_F32 && gt != OMK_F32 && gt != pt)
+        return learn_fail(OMK_ERR_UNSUPPORTED, "%s: 16-bit parameters with gradients of the other 16-bit type", who);
+    if (pt != OMK_F32 && ct != OMK_NONE)
+        return learn_fail(OMK_ERR_UNSUPPORTED, "%s: a copy is kept of 32-bit parameters only", who);
+    if (!(desc->beta1 >= 0.0 && desc->beta1 < 1.0) || !(desc->beta2 >= 0.0 && desc->beta2 < 1.0) || !(desc->eps >= 0.0) ||
+        !std::isfinite(desc->eps))
+        return learn_fail(OMK_ERR_INVALID, "%s: betas %g and %g (0 <= beta < 1), eps %g", who, desc->beta1, desc->beta2,
+                          desc->eps);
+    std::vector<AdamTensor> tensors((size_t)desc->n_tensors);
+    std::vector<int64_t> first_chunk((size_t)desc->n_tensors + 1, 0), elements((size_t)desc->n_tensors);
+    int64_t units = 0, n_chunks = 0;
+    for (int32_t i = 0; i < desc->n_tensors; i++) {
+        const omk_adamw_tensor &t = desc->h_tensors[i];
+        if (t.n < 0 || t.n > (int64_t)1 << 40) return learn_fail(OMK_ERR_INVALID, "%s: tensor %d of %lld elements", who, i, (long long)t.n);
+        if (!std::isfinite(t.lr_scale) || !std::isfinite(t.weight_decay))
+            return learn_fail(OMK_ERR_INVALID, "%s: tensor %d: lr_scale %g, weight_decay %g", who, i, t.lr_scale, t.weight_decay);
+        if (t.n && (!t.d_param || !t.d_m || !t.d_v || (ct != OMK_NONE && !t.d_copy) ||
+                    (st == OMK_F8 && (!t.d_m_scale || !t.d_v_scale))))
+            return learn_fail(OMK_ERR_INVALID, "%s: tensor %d: null argument", who, i);
+        if (ct == OMK_NONE && t.d_copy)
+            return learn_fail(OMK_ERR_INVALID, "%s: tensor %d has a copy, but copies have no type", who, i);
+        if (!aligned(t.d_param, width_of(pt)) || !aligned(t.d_copy, 2) || !aligned(t.d_m, width_of(st)) ||
+            !aligned(t.d_v, width_of(st)) || (st == OMK_F8 && (!aligned(t.d_m_scale, 4) || !aligned(t.d_v_scale, 4))))
+            return learn_fail(OMK_ERR_INVALID, "%s: tensor %d: an address that is no multiple of its type's size", who, i);
+        const int64_t own = (t.n + kUnit - 1) / kUnit;
+        tensors[i] = AdamTensor{t.n, t.d_param, t.d_copy, t.d_m, t.d_v, t.d_m_scale, t.d_v_scale, units,
+                                (float)t.lr_scale, (float)t.weight_decay};
+        elements[i] = t.n;
+        first_chunk[i] = n_chunks;
+        units += own;
+        n_chunks += (own + kChunkUnits - 1) / kChunkUnits;
+    }
+    first_chunk[(size_t)desc->n_tensors] = n_chunks;
+    if (units > UINT32_MAX || n_chunks > INT32_MAX)
+        return learn_fail(OMK_ERR_CAPACITY, "%s: over 2^40 elements", who);
+    std::vector<AdamChunk> chunks((size_t)n_chunks);
+    for (int32_t i = 0; i < desc->n_tensors; i++)
+        for (int64_t c = first_chunk[i]; c < first_chunk[i + 1]; c++)
+            chunks[(size_t)c] = AdamChunk{i, (int32_t)(c - first_chunk[i])};
+    omk_adamw *o = new (std::nothrow) omk_adamw();
+    if (!o) return learn_fail(OMK_ERR_INVALID, "out of host memory");
+    o->l = l;
+    l->children++;
+    o->n_tensors = desc->n_tensors;
+    o->param_type = pt;
+    o->grad_type = gt;
+    o->copy_type = ct;
+    o->state_type = st;
+    o->beta1 = desc->beta1;
+    o->beta2 = desc->beta2;
+    o->eps = desc->eps;
+    o->seed = desc->seed;
+    o->first_chunk.swap(first_chunk);
+    o->elements.swap(elements);
+    OnDevice on(l->device);
+    const size_t at_tensors = 256, at_chunks = at_tensors + (tensors.size() * sizeof(AdamTensor) + 255) / 256 * 256;
+    hipError_t e = on.status;
+    if (e == hipSuccess) e = hipMalloc((void **)&o->memory, at_chunks + chunks.size() * sizeof(AdamChunk) + 16);
+    if (e == hipSuccess) {
+        o->count = (AdamCount *)o->memory;
+        o->tensors = (AdamTensor *)(o->memory + at_tensors);
+        o->chunks = (AdamChunk *)(o->memory + at_chunks);
+        if (!tensors.empty())
+            e = hipMemcpy(o->tensors, tensors.data(), tensors.size() * sizeof(AdamTensor), hipMemcpyHostToDevice);
+    }
+    if (e == hipSuccess && !chunks.empty())
+        e = hipMemcpy(o->chunks, chunks.data(), chunks.size() * sizeof(AdamChunk), hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = launch_adamw_set(o->count, 0, 1.0, 1.0, l->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(l->stream);
+    if (e != hipSuccess) {
+        const int rc = learn_fail(OMK_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
+        omk_adamw_destroy(o);
+        return rc;
+    }
+    *out = o;
+    return OMK_OK;
+} LEARN_NO_THROW
+
+int omk_adamw_step(omk_adamw *o, const void *const *h_grads, double lr, const float *d_lr, const float *d_grad_scale) {
+    const char *who = "omk_adamw_step";
+    if (o && o->l->released) return learn_fail(OMK_ERR_STATE, "%s: the learner has been destroyed", who);
+    if (!o || (o->n_tensors && !h_grads)) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    if (!d_lr && !std::isfinite(lr)) return learn_fail(OMK_ERR_INVALID, "%s: lr %g", who, lr);
+    if (!aligned(d_lr, 4) || !aligned(d_grad_scale, 4))
+        return learn_fail(OMK_ERR_INVALID, "%s: an address that is no multiple of its type's size", who);
+    for (int32_t i = 0; i < o->n_tensors; i++)
+        if (!aligned(h_grads[i], width_of(o->grad_type)))
+            return learn_fail(OMK_ERR_INVALID, "%s: gradient %d at an address that is no multiple of its type's size", who, i);
+    OnDevice on(o->l->device);
+    LEARN_TRY(on.status);
+    AdamStep s;
+    s.tensors = o->tensors;
+    s.count = o->count;
+    s.d_lr = d_lr;
+    s.d_grad_scale = d_grad_scale;
+    s.lr = lr;
+    s.beta1 = o->beta1;
+    s.beta2 = o->beta2;
+    s.eps = (float)o->eps;
+    s.seed = o->seed;
+    for (int32_t t = 0; t == 0 || t < o->n_tensors; t += kGradsPerLaunch) {
+        const int32_t n = std::min(o->n_tensors - t, (int32_t)kGradsPerLaunch);
+        AdamGrads g;
+        memset(&g, 0, sizeof(g));
+        for (int32_t i = 0; i < n; i++) g.g[i] = h_grads[t + i];
+        s.first_tensor = t;
+        s.chunks = o->chunks + o->first_chunk[t];
+        s.n_chunks = o->first_chunk[t + n] - o->first_chunk[t];
+        s.last = t + kGradsPerLaunch >= o->n_tensors;
+        LEARN_TRY(launch_adamw(o->param_type, o->grad_type, o->copy_type, o->state_type, s, g, o->l->stream));
+    }
+    return OMK_OK;
+}
+
+int omk_adamw_set_steps(omk_adamw *o, int64_t steps) {
+    const char *who = "omk_adamw_set_steps";
+    if (!o) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    if (steps < 0 || steps > INT32_MAX) return learn_fail(OMK_ERR_INVALID, "%s: %lld steps", who, (long long)steps);
+    OnDevice on(o->l->device);
+    LEARN_TRY(on.status);
+    LEARN_TRY(launch_adamw_set(o->count, steps, std::pow(o->beta1, (double)steps), std::pow(o->beta2, (double)steps),
+                               o->l->stream));
+    return OMK_OK;
+}
+
+int omk_adamw_get_steps(omk_adamw *o, int64_t *h_steps) {
+    if (!o || !h_steps) return learn_fail(OMK_ERR_INVALID, "omk_adamw_get_steps: null argument");
+    OnDevice on(o->l->device);
+    LEARN_TRY(on.status);
+    AdamCount c;
+    LEARN_TRY(hipMemcpyAsync(&c, o->count, sizeof(c), hipMemcpyDeviceToHost, o->l->stream));
+    LEARN_TRY(hipStreamSynchronize(o->l->stream));
+    *h_steps = c.steps;
+    return OMK_OK;
+}
+
+}  // extern "C"

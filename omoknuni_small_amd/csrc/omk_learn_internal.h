@@ -1,0 +1,103 @@
+// What the translation units behind include/omk_learn.h share: arguments of the kernels, and their launchers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/omk_learn.h"
+
+namespace omk {
+
+// Sets the message of omk_last_error (omk_api.hip) and returns the code.
+int learn_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+
+struct Rows {
+    const void *x;
+    int64_t stride;
+    int64_t rows;
+    int32_t actions;
+    const uint32_t *legal;
+    int64_t legal_stride;
+};
+
+struct PolicyLoss {
+    const int32_t *moves;
+    const float *old_logprob, *advantage, *ref_logprob, *weight;
+    double log_low, log_high;  // borders of the ratio's logarithm
+    float low, high;           // borders of the ratio
+    float kl_weight, scale;
+    void *grad;
+    int64_t grad_stride;
+    float *logprob, *kl;
+    float *row_loss;  // work space: every row's share of the loss
+    float *loss;
+};
+
+struct PreferenceLoss {
+    const int32_t *moves, *line_begin;
+    int64_t pairs;
+    const float *ref_logprob;
+    float beta, smoothing, scale;
+    void *grad;
+    int64_t grad_stride;
+    int32_t zero_rest;
+    float *margin, *line_logprob, *loss;
+    // work space, per row: largest logit, one over the sum of exponentials, log-probability of the move (0: left out),
+    // derivative of the loss by it; per pair: its share of the loss
+    float *top, *inverse, *logprob, *slope, *pair_loss;
+};
+
+hipError_t launch_priors(int type, const Rows &r, float *priors, int64_t prior_stride, hipStream_t stream);
+hipError_t launch_logprobs(int type, const Rows &r, const int32_t *moves, float *logprob, float *entropy,
+                           hipStream_t stream);
+hipError_t launch_policy_loss(int type, const Rows &r, const PolicyLoss &p, hipStream_t stream);
+hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss &p, hipStream_t stream);
+hipError_t launch_set_float(float *to, float value, hipStream_t stream);
+
+constexpr int kUnit = 256;      // elements that share a scale, and that a wavefront steps at a time
+constexpr int kChunkUnits = 8;  // units of a chunk: what a block takes at a time, all of one tensor
+constexpr int kGradsPerLaunch = 256;  // gradient pointers that travel as kernel arguments
+
+struct AdamTensor {
+    int64_t n;
+    void *param, *copy, *m, *v;
+    float *m_scale, *v_scale;
+    int64_t first_unit;  // units of the tensors before it
+    float lr_scale, weight_decay;
+};
+
+struct AdamChunk {
+    int32_t tensor;
+    int32_t chunk;  // of the tensor's
+};
+
+// Lives on the device: steps done, beta1^steps, beta2^steps, and the blocks of the running step that are done.
+struct AdamCount {
+    double power1, power2;
+    int64_t steps;
+    uint32_t done, reserved;
+};
+
+struct AdamGrads {
+    const void *g[kGradsPerLaunch];
+};
+
+struct AdamStep {
+    const AdamTensor *tensors;
+    const AdamChunk *chunks;
+    int64_t n_chunks;
+    int32_t first_tensor;
+    AdamCount *count;
+    const float *d_lr, *d_grad_scale;
+    double lr;
+    double beta1, beta2;
+    float eps;
+    uint32_t seed;
+    int32_t last;  // this launch ends the step
+};
+
+hipError_t launch_adamw(int param, int grad, int copy, int state, const AdamStep &s, const AdamGrads &g,
+                        hipStream_t stream);
+hipError_t launch_adamw_set(AdamCount *count, int64_t steps, double power1, double power2, hipStream_t stream);
+
+}  // namespace omk
