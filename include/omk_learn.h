@@ -65,15 +65,20 @@ typedef struct omk_policy_rows {
     int64_t legal_stride;    /* words between two rows' masks; 0: one mask for all rows */
 } omk_policy_rows;
 
+/* Bytes of d_work that the two calls below need: 0 (and d_work may be NULL) for rows of up to 65528 actions.  Work
+ * space lies at a multiple of 16 bytes; the same memory may serve calls one after another on a stream. */
+int64_t omk_policy_work(int64_t rows, int32_t actions);
+
 /* Probabilities of the actions, in 32 bits: d_priors[r * prior_stride + j].  What omk_expand_batch takes as
  * h_policy.  d_priors must not overlap the logits. */
-int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride);
+int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride, void *d_work,
+                      int64_t work_bytes);
 
 /* d_logprob[r] = log-probability of the move d_moves[r]: 0 where the move lies outside [0, actions), -inf where it
  * is not legal or the row has no policy.  d_entropy[r] = -sum p log p.  Either output may be NULL (d_moves too, then,
  * when d_logprob is). */
 int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32_t *d_moves, float *d_logprob,
-                        float *d_entropy);
+                        float *d_entropy, void *d_work, int64_t work_bytes);
 
 /* Clipped policy loss with a KL term.  Row by row, with lp = log p(move):
  *   ratio = exp(lp - old_logprob)
@@ -101,7 +106,7 @@ typedef struct omk_policy_loss_out {
     float *d_logprob;    /* [rows]; 0 in rows left out */
     float *d_kl;         /* [rows]; 0 in rows left out; NULL allowed */
 } omk_policy_loss_out;
-/* Bytes of d_work for this many rows (the same memory may serve calls one after another on a stream). */
+/* Bytes of d_work for this many rows. */
 int64_t omk_policy_loss_work(int64_t rows, int32_t actions);
 int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_policy_samples *samples,
                     const omk_policy_loss_params *params, const omk_policy_loss_out *out, void *d_work,

@@ -92,7 +92,8 @@ int check_rows(const char *who, const omk_policy_rows *r, Rows *out) {
     if (r->rows && (span_bytes(r->rows, r->row_stride, r->actions, width_of(r->type)) < 0 ||
                     (r->d_legal && span_bytes(r->rows, r->legal_stride, words, 4) < 0)))
         return learn_fail(OMK_ERR_INVALID, "%s: rows that pass the address space", who);
-    *out = Rows{r->d_logits, r->row_stride, r->rows, r->actions, r->d_legal, r->legal_stride};
+    *out = Rows{r->d_logits, r->row_stride, r->rows, r->actions, r->d_legal, r->legal_stride, words,
+                r->rows ? (r->rows - 1) * r->row_stride + r->actions : 0, aligned(r->d_logits, 16)};
     return OMK_OK;
 }
 
@@ -109,6 +110,14 @@ int check_result(const char *who, const char *what, const omk_policy_rows *r, co
     if (in_place && d == r->d_logits && (r->rows < 2 || stride == r->row_stride)) return OMK_OK;
     if (overlap(d, bytes, r->d_logits, of_logits))
         return learn_fail(OMK_ERR_INVALID, "%s: the %s lies across the logits", who, what);
+    return OMK_OK;
+}
+
+int check_work(const char *who, const void *d_work, int64_t work_bytes, int64_t needed) {
+    if (!aligned(d_work, 16)) return learn_fail(OMK_ERR_INVALID, "%s: work space at an address that is no multiple of 16", who);
+    if (needed && (!d_work || work_bytes < needed))
+        return learn_fail(OMK_ERR_CAPACITY, "%s: %lld bytes of work space, %lld needed", who,
+                          (long long)(d_work ? work_bytes : 0), (long long)needed);
     return OMK_OK;
 }
 
@@ -166,21 +175,25 @@ int omk_learner_sync(omk_learner *l) {
     return OMK_OK;
 }
 
-int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride) {
+int64_t omk_policy_work(int64_t rows, int32_t actions) { return rows > 0 ? wide_work(rows, actions) : 0; }
+
+int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride, void *d_work,
+                      int64_t work_bytes) {
     const char *who = "omk_policy_priors";
     if (!l || !rows) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
     Rows r;
     if (int rc = check_rows(who, rows, &r)) return rc;
     if (!r.rows) return OMK_OK;
     if (int rc = check_result(who, "priors", rows, d_priors, prior_stride, 4, false)) return rc;
+    if (int rc = check_work(who, d_work, work_bytes, omk_policy_work(r.rows, r.actions))) return rc;
     OnDevice on(l->device);
     LEARN_TRY(on.status);
-    LEARN_TRY(launch_priors(rows->type, r, d_priors, prior_stride, l->stream));
+    LEARN_TRY(launch_priors(rows->type, r, d_priors, prior_stride, d_work, l->stream));
     return OMK_OK;
 }
 
 int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32_t *d_moves, float *d_logprob,
-                        float *d_entropy) {
+                        float *d_entropy, void *d_work, int64_t work_bytes) {
     const char *who = "omk_policy_logprobs";
     if (!l || !rows) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
     Rows r;
@@ -189,15 +202,15 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
     const void *all[] = {d_moves, d_logprob, d_entropy};
     if (!aligned4(who, all, 3)) return OMK_ERR_INVALID;
     if (!r.rows || (!d_logprob && !d_entropy)) return OMK_OK;
+    if (int rc = check_work(who, d_work, work_bytes, omk_policy_work(r.rows, r.actions))) return rc;
     OnDevice on(l->device);
     LEARN_TRY(on.status);
-    LEARN_TRY(launch_logprobs(rows->type, r, d_moves, d_logprob, d_entropy, l->stream));
+    LEARN_TRY(launch_logprobs(rows->type, r, d_moves, d_logprob, d_entropy, d_work, l->stream));
     return OMK_OK;
 }
 
 int64_t omk_policy_loss_work(int64_t rows, int32_t actions) {
-    (void)actions;
-    return rows > 0 ? rows * 4 : 0;
+    return rows > 0 ? (rows * 4 + 15) / 16 * 16 + wide_work(rows, actions) : 0;
 }
 
 int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_policy_samples *samples,
@@ -215,18 +228,15 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
         return learn_fail(OMK_ERR_INVALID, "%s: a KL term needs the reference's log-probabilities", who);
     if (!out->d_loss) return learn_fail(OMK_ERR_INVALID, "%s: no loss", who);
     const void *all[] = {samples->d_moves, samples->d_old_logprob, samples->d_advantage, samples->d_ref_logprob,
-                         samples->d_weight, out->d_loss, out->d_logprob, out->d_kl, d_work};
-    if (!aligned4(who, all, 9)) return OMK_ERR_INVALID;
+                         samples->d_weight, out->d_loss, out->d_logprob, out->d_kl};
+    if (!aligned4(who, all, 8)) return OMK_ERR_INVALID;
     if (r.rows) {
         if (!samples->d_moves || !samples->d_old_logprob || !samples->d_advantage || !out->d_logprob)
             return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
         if (out->d_grad)
             if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
                 return rc;
-        const int64_t needed = omk_policy_loss_work(r.rows, r.actions);
-        if (needed && (!d_work || work_bytes < needed))
-            return learn_fail(OMK_ERR_CAPACITY, "%s: %lld bytes of work space, %lld needed", who,
-                              (long long)(d_work ? work_bytes : 0), (long long)needed);
+        if (int rc = check_work(who, d_work, work_bytes, omk_policy_loss_work(r.rows, r.actions))) return rc;
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);
@@ -250,15 +260,19 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
     p.grad_stride = out->grad_stride;
     p.logprob = out->d_logprob;
     p.kl = out->d_kl;
-    p.row_loss = (float *)d_work;
+    p.shares = (float *)d_work;
     p.loss = out->d_loss;
     LEARN_TRY(launch_policy_loss(rows->type, r, p, l->stream));
     return OMK_OK;
 }
 
+// 20 bytes a row and 4 a pair
+static int64_t preference_before(int64_t rows, int64_t pairs) {
+    return ((rows > 0 ? rows * 20 : 0) + (pairs > 0 ? pairs * 4 : 0) + 15) / 16 * 16;
+}
+
 int64_t omk_preference_loss_work(int64_t rows, int32_t actions, int64_t pairs) {
-    (void)actions;
-    return (rows > 0 ? rows * 16 : 0) + (pairs > 0 ? pairs * 4 : 0);
+    return preference_before(rows, pairs) + (rows > 0 ? wide_work(rows, actions) : 0);
 }
 
 int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32_t *d_moves,
@@ -275,17 +289,14 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
         return learn_fail(OMK_ERR_INVALID, "%s: beta %g, label_smoothing %g (0 .. 0.5), scale %g", who, params->beta,
                           params->label_smoothing, params->scale);
     if (!out->d_loss) return learn_fail(OMK_ERR_INVALID, "%s: no loss", who);
-    const void *all[] = {d_moves, d_line_begin, d_ref_logprob, out->d_loss, out->d_margin, out->d_line_logprob, d_work};
-    if (!aligned4(who, all, 7)) return OMK_ERR_INVALID;
+    const void *all[] = {d_moves, d_line_begin, d_ref_logprob, out->d_loss, out->d_margin, out->d_line_logprob};
+    if (!aligned4(who, all, 6)) return OMK_ERR_INVALID;
     if (pairs) {
         if (!d_line_begin || (r.rows && !d_moves)) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
         if (r.rows && out->d_grad)
             if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
                 return rc;
-        const int64_t needed = omk_preference_loss_work(r.rows, r.actions, pairs);
-        if (!d_work || work_bytes < needed)
-            return learn_fail(OMK_ERR_CAPACITY, "%s: %lld bytes of work space, %lld needed", who,
-                              (long long)(d_work ? work_bytes : 0), (long long)needed);
+        if (int rc = check_work(who, d_work, work_bytes, omk_preference_loss_work(r.rows, r.actions, pairs))) return rc;
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);
@@ -307,13 +318,13 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
     p.margin = out->d_margin;
     p.line_logprob = out->d_line_logprob;
     p.loss = out->d_loss;
-    float *work = (float *)d_work;
-    p.top = work;
-    p.inverse = work + r.rows;
-    p.logprob = work + 2 * r.rows;
-    p.slope = work + 3 * r.rows;
-    p.pair_loss = work + 4 * r.rows;
-    LEARN_TRY(launch_preference_loss(rows->type, r, p, l->stream));
+    p.work = d_work;
+    p.logprob = (double *)d_work;
+    p.top = (float *)(p.logprob + r.rows);
+    p.inverse = p.top + r.rows;
+    p.slope = p.inverse + r.rows;
+    p.pair_loss = p.slope + r.rows;
+    LEARN_TRY(launch_preference_loss(rows->type, r, p, preference_before(r.rows, pairs), l->stream));
     return OMK_OK;
 }
 

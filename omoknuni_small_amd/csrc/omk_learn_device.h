@@ -17,38 +17,89 @@ constexpr double kLn2 = 0.693147180559945309417;
 // exp(x) itself that gets small.  Below 2^-126 the result may be flushed to 0: 1e-38 of the largest term.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
 
-// log(s) in 64 bits from a 32-bit sum: the exponent is taken off, so that what is rounded is the logarithm of a number
-// near 1.  (A loss compares a ratio with borders: the log-probability keeps more than the 24 bits of one float.)
-__device__ __forceinline__ double log_of_sum(float s) {
-    int k = __builtin_amdgcn_frexp_expf(s);
-    float f = __builtin_amdgcn_frexp_mantf(s);  // [0.5, 1)
-    if (f < 0.70710678f) {
-        f *= 2.0f;
-        k--;
+// A reduction over teams of 8 .. 64 neighbouring lanes, the result in every lane of the team: lanes of a row of 16 by quad
+// swaps and mirrors, rows and halves by exchanging them.  (All 64 lanes are active where these are called.)
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, true);
+    return __hiloint2double(hi, lo);
+}
+struct Two {
+    uint32_t a, b;
+};
+__device__ __forceinline__ Two swap16(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
+__device__ __forceinline__ Two swap32(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
+
+template <int TEAM>
+__device__ __forceinline__ float team_max(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp_f32<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp_f32<0x141>(v));  // row_half_mirror
+    if (TEAM > 8) v = fmaxf(v, dpp_f32<0x140>(v));  // row_mirror
+    if (TEAM > 16) {
+        const Two r = swap16(__float_as_uint(v));
+        v = fmaxf(__uint_as_float(r.a), __uint_as_float(r.b));
     }
-    return (double)k * kLn2 + (double)logf(f);
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    if (TEAM > 32) {
+        const Two r = swap32(__float_as_uint(v));
+        v = fmaxf(__uint_as_float(r.a), __uint_as_float(r.b));
+    }
     return v;
 }
 
-// What a row comes to: largest legal logit, sum of exp(x - top) over the legal ones (0: no policy), sum of
-// exp(x - top) (x - top).
-struct RowStats {
-    float top, sum, centred;
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v) {
+    v += dpp_f32<0xB1>(v);
+    v += dpp_f32<0x4E>(v);
+    v += dpp_f32<0x141>(v);
+    if (TEAM > 8) v += dpp_f32<0x140>(v);
+    if (TEAM > 16) {
+        const Two r = swap16(__float_as_uint(v));
+        v = __uint_as_float(r.a) + __uint_as_float(r.b);
+    }
+    if (TEAM > 32) {
+        const Two r = swap32(__float_as_uint(v));
+        v = __uint_as_float(r.a) + __uint_as_float(r.b);
+    }
+    return v;
+}
+
+template <int TEAM>
+__device__ __forceinline__ double team_sum(double v) {
+    v += dpp_f64<0xB1>(v);
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x141>(v);
+    if (TEAM > 8) v += dpp_f64<0x140>(v);
+    if (TEAM > 16) {
+        const Two lo = swap16((uint32_t)__double2loint(v)), hi = swap16((uint32_t)__double2hiint(v));
+        v = __hiloint2double((int)hi.a, (int)lo.a) + __hiloint2double((int)hi.b, (int)lo.b);
+    }
+    if (TEAM > 32) {
+        const Two lo = swap32((uint32_t)__double2loint(v)), hi = swap32((uint32_t)__double2hiint(v));
+        v = __hiloint2double((int)hi.a, (int)lo.a) + __hiloint2double((int)hi.b, (int)lo.b);
+    }
+    return v;
+}
+
+// 16 bytes of a matrix, as numbers.
+template <typename T>
+struct Pack {
+    static constexpr int V = 16 / (int)sizeof(T);
+    union {
+        uint4 raw;
+        T x[V];
+    };
 };
 
 }  // namespace omk

@@ -18,7 +18,15 @@ struct Rows {
     int32_t actions;
     const uint32_t *legal;
     int64_t legal_stride;
+    int32_t words;  // of a row's mask
+    int64_t span;   // elements from the first to behind the last
+    bool aligned;   // the first lies at a multiple of 16 bytes
 };
+
+// Rows of up to this many actions are held in registers, whatever their type and alignment (65536 and up to 7 elements
+// before the row, in the widest team); wider ones need work space.
+constexpr int32_t kMostInRegisters = 65536 - 8;
+int64_t wide_work(int64_t rows, int32_t actions);  // bytes
 
 struct PolicyLoss {
     const int32_t *moves;
@@ -29,7 +37,7 @@ struct PolicyLoss {
     void *grad;
     int64_t grad_stride;
     float *logprob, *kl;
-    float *row_loss;  // work space: every row's share of the loss
+    float *shares;  // work space: the blocks' shares of the loss (at most one a row), and what wide rows need
     float *loss;
 };
 
@@ -42,16 +50,19 @@ struct PreferenceLoss {
     int64_t grad_stride;
     int32_t zero_rest;
     float *margin, *line_logprob, *loss;
-    // work space, per row: largest logit, one over the sum of exponentials, log-probability of the move (0: left out),
-    // derivative of the loss by it; per pair: its share of the loss
-    float *top, *inverse, *logprob, *slope, *pair_loss;
+    // work space, per row: log-probability of the move (0: left out), largest logit, one over the sum of exponentials,
+    // derivative of the loss by the log-probability; per pair: its share of the loss; and what wide rows need
+    void *work;
+    double *logprob;
+    float *top, *inverse, *slope, *pair_loss;
 };
 
-hipError_t launch_priors(int type, const Rows &r, float *priors, int64_t prior_stride, hipStream_t stream);
-hipError_t launch_logprobs(int type, const Rows &r, const int32_t *moves, float *logprob, float *entropy,
+hipError_t launch_priors(int type, const Rows &r, float *priors, int64_t prior_stride, void *work, hipStream_t stream);
+hipError_t launch_logprobs(int type, const Rows &r, const int32_t *moves, float *logprob, float *entropy, void *work,
                            hipStream_t stream);
 hipError_t launch_policy_loss(int type, const Rows &r, const PolicyLoss &p, hipStream_t stream);
-hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss &p, hipStream_t stream);
+// before: bytes of its work space that come before what wide rows need
+hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss &p, int64_t before, hipStream_t stream);
 hipError_t launch_set_float(float *to, float value, hipStream_t stream);
 
 constexpr int kUnit = 256;      // elements that share a scale, and that a wavefront steps at a time

@@ -1,0 +1,661 @@
+// Kernels over rows of logits.  What they all compute, per row: m = max over the legal x, S = sum exp(x - m); then an
+// operator's few numbers per row, and from exp(x - m) its output per element.  k_rows reads every row once: a team of
+// lanes holds it in registers from the look for its largest logit to the writing of its gradient (or priors).
+// Rows too wide for that are cut into pieces (k_parts, k_apply) and read twice.
+// Instantiated per type of the logits by omk_policy_{f32,bf16,f16}.hip.
+#pragma once
+
+#include "omk_learn_device.h"
+#include "omk_learn_internal.h"
+
+namespace omk {
+
+// What a row (or a part of one) comes to: its largest legal logit (0 if there is none), the sum of exp(x - top) (x - top)
+// over the legal ones, and the sum of exp(x - top) (0: no policy).
+struct RowStats {
+    float top, centred;
+    double sum;
+};
+
+// log(s) in 64 bits: the exponent is taken off, so that what is rounded is the logarithm of a number near 1.  (A loss
+// compares a ratio with borders: the log-probability keeps more than the 24 bits of a float.)
+__device__ __forceinline__ double log_of_sum(double s) {
+    int k = __builtin_amdgcn_frexp_exp(s);
+    double f = __builtin_amdgcn_frexp_mant(s);  // [0.5, 1)
+    if (f < 0.70710678) {
+        f *= 2.0;
+        k--;
+    }
+    const float near = (float)f;
+    return (double)k * kLn2 + (double)(logf(near) + (float)(f - (double)near) / near);
+}
+
+// ---- 16 bytes of a row ----
+
+// Vectors of a row lie at multiples of 16 bytes of the matrix, not of the row: the first holds `head` elements of what
+// lies before the row, so that rows of any width are read by whole vectors.  (Without `aligned`: rows are cut from
+// their first element, and vectors are put together element by element.)
+template <typename T>
+__device__ __forceinline__ int head_of(const Rows &r, int64_t row) {
+    return r.aligned ? (int)((uint64_t)(row * r.stride) & (Pack<T>::V - 1)) : 0;
+}
+
+// Bits of the elements j .. j + V - 1 that are the row's.
+template <int V>
+__device__ __forceinline__ uint32_t inside_bits(int j, int actions) {
+    uint32_t b = (1u << V) - 1u;
+    if (j < 0) b &= b << -j;
+    if (j + V > actions) b = j < actions ? b & ((1u << (actions - j)) - 1u) : 0u;
+    return b;
+}
+
+// Bits of the elements that are legal (of those that are the row's).
+__device__ __forceinline__ uint32_t legal_bits(const uint32_t *legal, int words, int j) {
+    const int at = j < 0 ? 0 : j, w = at >> 5;
+    const uint32_t lo = legal[min(w, words - 1)], hi = legal[min(w + 1, words - 1)];
+    const uint32_t bits = __builtin_amdgcn_alignbit(hi, lo, at & 31);
+    return j < 0 ? bits << -j : bits;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_vector(const Rows &r, int64_t row, int j, uint32_t inside, Pack<T> &p) {
+    constexpr int V = Pack<T>::V;
+    const int64_t at = row * r.stride + j;
+    if (!inside) return;
+    if (r.aligned && at + V <= r.span) {  // (at >= 0: the matrix begins at a multiple of 16 bytes)
+        p.raw = *(const uint4 *)((const T *)r.x + at);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (inside >> i & 1u) p.x[i] = ((const T *)r.x)[at + i];
+}
+
+template <typename T, typename OUT>
+__device__ __forceinline__ void store_vector(OUT *out, bool aligned, int j, int actions, const float (&y)[Pack<T>::V]) {
+    constexpr int V = Pack<T>::V;
+    if (aligned && j >= 0 && j + V <= actions) {
+        if constexpr (sizeof(OUT) == sizeof(T)) {
+            Pack<OUT> p;
+#pragma unroll
+            for (int i = 0; i < V; i++) p.x[i] = (OUT)y[i];
+            *(uint4 *)(out + j) = p.raw;
+        } else {  // 32-bit results of 16-bit logits
+#pragma unroll
+            for (int i = 0; i < V; i += 4) *(float4 *)(out + j + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (j + i >= 0 && j + i < actions) out[j + i] = (OUT)y[i];
+}
+
+template <int V>
+__device__ __forceinline__ float sum_of(const float (&e)[V]) {
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i] = e[i];
+#pragma unroll
+    for (int d = V / 2; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < d; i++) s[i] += s[i + d];
+    return s[0];
+}
+
+// ---- what operators do with a row ----
+
+// The move of a row (-1 where it lies outside the action space) and its logit, -inf where it is not legal.
+struct Move {
+    int32_t move;
+    float chosen;
+};
+template <typename T>
+__device__ __forceinline__ Move move_of(const Rows &r, const int32_t *moves, int64_t row) {
+    Move m = {moves ? moves[row] : -1, -INFINITY};
+    if ((uint32_t)m.move >= (uint32_t)r.actions) m.move = -1;
+    if (m.move >= 0 && (!r.legal || (r.legal[row * r.legal_stride + (m.move >> 5)] >> (m.move & 31) & 1u)))
+        m.chosen = (float)((const T *)r.x)[row * r.stride + m.move];
+    return m;
+}
+
+// The result of an operator's look at a row: element j becomes each * exp(x_j - top), and at_move more where j is the
+// move; 0 wherever `none`.
+struct RowOut {
+    float each, at_move;
+    int32_t move;
+    bool none;
+    float share;  // of the loss
+};
+
+struct PriorsOp {
+    static constexpr bool kCentred = false, kElements = true, kMoves = false, kLoss = false;
+    template <typename T>
+    using Element = float;
+    const int32_t *moves;  // nullptr
+    float *block_loss;     // nullptr
+    float *priors;
+    int64_t stride;
+    bool aligned;
+    template <typename OUT>
+    __device__ OUT *elements(int64_t row) const {
+        return priors + row * stride;
+    }
+    __device__ RowOut row(int64_t, const RowStats &s, Move, bool) const {
+        return {s.sum == 0.0 ? 0.0f : 1.0f / (float)s.sum, 0.0f, -1, s.sum == 0.0, 0.0f};
+    }
+};
+
+struct LogprobsOp {
+    static constexpr bool kCentred = true, kElements = false, kMoves = true, kLoss = false;
+    const int32_t *moves;
+    float *block_loss;  // nullptr
+    float *logprob, *entropy;
+    __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
+        if (writes) {
+            const double log_sum = log_of_sum(s.sum);
+            if (entropy) entropy[row] = s.sum == 0.0 ? 0.0f : (float)(log_sum - (double)(s.centred / (float)s.sum));
+            if (logprob)
+                logprob[row] = m.move < 0       ? 0.0f
+                               : s.sum == 0.0 ? -INFINITY
+                                              : (float)((double)m.chosen - (double)s.top - log_sum);
+        }
+        return {0.0f, 0.0f, -1, true, 0.0f};
+    }
+};
+
+// exp(d) - d - 1 without the cancellation near 0: d^2/2 (1 + d/3 (1 + d/4 (..))), whose first term left out is below
+// 2^-24 of the sum for |d| < 1/4
+__device__ __forceinline__ float exp_minus_linear(float d, float expm1_d) {
+    if (fabsf(d) >= 0.25f) return expm1_d - d;
+    float s = 1.0f + d * (1.0f / 9.0f);
+    s = 1.0f + d * (1.0f / 8.0f) * s;
+    s = 1.0f + d * (1.0f / 7.0f) * s;
+    s = 1.0f + d * (1.0f / 6.0f) * s;
+    s = 1.0f + d * (1.0f / 5.0f) * s;
+    s = 1.0f + d * (1.0f / 4.0f) * s;
+    s = 1.0f + d * (1.0f / 3.0f) * s;
+    return 0.5f * d * d * s;
+}
+
+struct PolicyOp {
+    static constexpr bool kCentred = false, kElements = true, kMoves = true, kLoss = true;
+    template <typename T>
+    using Element = T;
+    const int32_t *moves;
+    float *block_loss;  // a block's share of the loss, by the block's number (by the row where rows are cut)
+    PolicyLoss p;
+    bool aligned;
+    template <typename OUT>
+    __device__ OUT *elements(int64_t row) const {
+        return p.grad ? (OUT *)p.grad + row * p.grad_stride : nullptr;
+    }
+    __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
+        float lp = 0.0f, kl = 0.0f, loss = 0.0f, slope = 0.0f;
+        if (m.chosen != -INFINITY) {
+            const double exact = (double)m.chosen - (double)s.top - log_of_sum(s.sum);
+            lp = (float)exact;
+            const float a = p.advantage[row];
+            const double shift = exact - (double)p.old_logprob[row];
+            if (a > 0.0f ? shift > p.log_high : a < 0.0f && shift < p.log_low) {
+                loss = -(a > 0.0f ? p.high : p.low) * a;
+            } else if (a != 0.0f) {
+                loss = slope = -expf((float)shift) * a;
+            }
+            if (p.ref_logprob) {
+                const float d = (float)((double)p.ref_logprob[row] - exact), e = expm1f(d);
+                kl = exp_minus_linear(d, e);
+                loss += p.kl_weight * kl;
+                slope -= p.kl_weight * e;
+            }
+            const float w = (p.weight ? p.weight[row] : 1.0f) * p.scale;
+            loss *= w;
+            slope *= w;
+        }
+        if (writes) {
+            p.logprob[row] = lp;
+            if (p.kl) p.kl[row] = kl;
+        }
+        return {slope == 0.0f ? 0.0f : -slope / (float)s.sum, slope, m.move, slope == 0.0f, loss};
+    }
+};
+
+struct LineOp {
+    static constexpr bool kCentred = false, kElements = false, kMoves = true, kLoss = false;
+    const int32_t *moves;
+    float *block_loss;  // nullptr
+    PreferenceLoss p;
+    __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
+        if (writes) {
+            const bool counts = m.chosen != -INFINITY;
+            p.top[row] = s.top;
+            p.inverse[row] = counts ? 1.0f / (float)s.sum : 0.0f;
+            p.logprob[row] = counts ? (double)m.chosen - (double)s.top - log_of_sum(s.sum) : 0.0;
+            p.slope[row] = 0.0f;  // until its line says otherwise
+        }
+        return {0.0f, 0.0f, -1, true, 0.0f};
+    }
+};
+
+// The rows that lines hold: line_begin's first to its last, inside the rows there are.
+struct LineRows {
+    int64_t begin, end;
+};
+__device__ __forceinline__ int64_t inside_rows(int64_t at, int64_t rows) { return at < 0 ? 0 : at > rows ? rows : at; }
+__device__ __forceinline__ LineRows line_rows(const PreferenceLoss &p, int64_t rows) {
+    return {inside_rows(p.line_begin[0], rows), inside_rows(p.line_begin[2 * p.pairs], rows)};
+}
+
+// ---- rows that registers hold ----
+
+// Joins the maxima and sums of a block's wavefronts, whose terms are relative to their own maxima until then: one
+// exchange through LDS serves both.  Every thread of the block calls it; the result is the same in all of them.
+template <bool CENTRED, int WAVES>
+__device__ __forceinline__ RowStats join_waves(float top, double sum, float centred) {
+    __shared__ float tops[WAVES], centreds[WAVES];
+    __shared__ double sums[WAVES];
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        tops[wave] = top;
+        sums[wave] = sum;
+        if (CENTRED) centreds[wave] = centred;
+    }
+    __syncthreads();
+    RowStats all = {-INFINITY, 0.0f, 0.0};
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) all.top = fmaxf(all.top, tops[w]);
+    if (all.top == -INFINITY) all.top = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        const bool empty = tops[w] == -INFINITY;  // (its sum is 0, or NaN)
+        const float d = empty ? 0.0f : tops[w] - all.top, f = exp_of(d);
+        all.sum += sums[w] * (double)f;
+        if (CENTRED) all.centred += (centreds[w] + (float)sums[w] * d) * f;
+    }
+    return all;
+}
+
+// TEAM lanes hold a row, K vectors each.  Up to 64 lanes: blocks of 256 threads, whose teams take rows of their
+// own; more: a block a row.
+template <typename T, int TEAM, int K, typename OP>
+__global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void k_rows(Rows r, OP op) {
+    constexpr int V = Pack<T>::V;
+    constexpr int BLOCK = TEAM <= 64 ? 256 : TEAM, WAVES = BLOCK / 64, LANES = TEAM < 64 ? TEAM : 64;
+    constexpr bool KEEP = K * V <= 32;  // exp(x - m) stays in registers; wider rows compute it again from the logits
+    const int sub = threadIdx.x & (TEAM - 1);
+    const int64_t row = TEAM <= 64 ? (int64_t)blockIdx.x * (BLOCK / TEAM) + threadIdx.x / TEAM : (int64_t)blockIdx.x;
+    const bool here = row < r.rows;
+    const int head = here ? head_of<T>(r, row) : 0;
+
+    // (the wavefront that looks at the move writes no other's part of the row before it has used what it found: the
+    // gradient may lie where the logits are)
+    Move m = {-1, -INFINITY};
+    if (OP::kMoves && here && (TEAM <= 64 || threadIdx.x < 64)) m = move_of<T>(r, op.moves, row);
+    Pack<T> p[K];
+    uint32_t bits[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int j = (k * TEAM + sub) * V - head;
+        bits[k] = here ? inside_bits<V>(j, r.actions) : 0u;
+        load_vector<T>(r, row, j, bits[k], p[k]);
+    }
+    if (r.legal && here) {
+        const uint32_t *legal = r.legal + row * r.legal_stride;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (bits[k]) bits[k] &= legal_bits(legal, r.words, (k * TEAM + sub) * V - head);
+    }
+    const auto logit = [&](int k, int i) { return bits[k] >> i & 1u ? (float)p[k].x[i] : -INFINITY; };
+
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) top = fmaxf(top, logit(k, i));
+    top = team_max<LANES>(top);
+    const float own_top = top == -INFINITY ? 0.0f : top;
+    float e[KEEP ? K : 1][V];
+    float sum = 0.0f, centred = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        float t[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float d = logit(k, i) - own_top;
+            t[i] = exp_of(d);
+            if (OP::kCentred) centred += t[i] > 0.0f ? t[i] * d : 0.0f;
+            if (KEEP) e[k][i] = t[i];
+        }
+        sum += sum_of<V>(t);
+    }
+    RowStats s = {own_top, 0.0f, team_sum<LANES>((double)sum)};
+    if (OP::kCentred) s.centred = team_sum<LANES>(centred);
+
+    float factor = 1.0f;  // from this wavefront's maximum to the row's
+    RowOut out;
+    if constexpr (TEAM <= 64) {
+        out = op.row(here ? row : 0, s, m, here && sub == 0);
+    } else {
+        __shared__ RowOut shared_out;
+        s = join_waves<OP::kCentred, WAVES>(top, s.sum, s.centred);
+        factor = top == -INFINITY ? 0.0f : exp_of(top - s.top);
+        if (threadIdx.x < 64) {
+            out = op.row(row, s, m, threadIdx.x == 0);
+            if (threadIdx.x == 0) shared_out = out;
+        }
+        if (OP::kElements) {
+            __syncthreads();
+            out = shared_out;
+        }
+    }
+
+    if constexpr (OP::kElements) {
+        typedef typename OP::template Element<T> OUT;
+        OUT *to = op.template elements<OUT>(row);
+        if (to && here) {
+            const float each = out.each * factor;
+            const int at = out.move < 0 ? -1 : out.move + head;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int vec = k * TEAM + sub, j = vec * V - head;
+                if (j >= r.actions) continue;
+                float y[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float t = KEEP ? e[k][i] : exp_of(logit(k, i) - own_top);
+                    y[i] = out.none ? 0.0f : t * each;
+                }
+                if (at >= 0 && at / V == vec) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) y[i] += at % V == i ? out.at_move : 0.0f;
+                }
+                store_vector<T, OUT>(to, op.aligned, j, r.actions, y);
+            }
+        }
+    }
+
+    if constexpr (OP::kLoss) {
+        if constexpr (TEAM <= 64) {
+            __shared__ float shares[BLOCK / TEAM];
+            if (sub == 0) shares[threadIdx.x / TEAM] = here ? out.share : 0.0f;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                double all = 0.0;
+                for (int i = 0; i < BLOCK / TEAM; i++) all += (double)shares[i];
+                op.block_loss[blockIdx.x] = (float)all;
+            }
+        } else if (threadIdx.x == 0) {
+            op.block_loss[blockIdx.x] = out.share;
+        }
+    }
+}
+
+// ---- rows cut into pieces ----
+
+constexpr int kPieceBlock = 256;
+constexpr int kPieceVectors = 8;  // of a thread
+
+template <typename T>
+__host__ __device__ constexpr int piece_elements() {
+    return kPieceBlock * kPieceVectors * Pack<T>::V;
+}
+
+struct Wide {
+    int32_t pieces;
+    RowStats *parts;  // [rows][pieces]
+    Move *moves;      // [rows]: looked up before any gradient is written where logits may be
+};
+
+template <typename T, typename OP>
+__global__ __launch_bounds__(kPieceBlock) void k_parts(Rows r, OP op, Wide w) {
+    constexpr int V = Pack<T>::V, K = kPieceVectors;
+    const int64_t row = blockIdx.x / w.pieces;
+    const int piece = blockIdx.x % w.pieces, head = head_of<T>(r, row);
+    const int first = piece * (K * kPieceBlock) + threadIdx.x;
+    Pack<T> p[K];
+    uint32_t bits[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int j = (first + k * kPieceBlock) * V - head;
+        bits[k] = inside_bits<V>(j, r.actions);
+        load_vector<T>(r, row, j, bits[k], p[k]);
+        if (r.legal && bits[k]) bits[k] &= legal_bits(r.legal + row * r.legal_stride, r.words, j);
+    }
+    const auto logit = [&](int k, int i) { return bits[k] >> i & 1u ? (float)p[k].x[i] : -INFINITY; };
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) top = fmaxf(top, logit(k, i));
+    top = team_max<64>(top);
+    const float own_top = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, centred = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        float t[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float d = logit(k, i) - own_top;
+            t[i] = exp_of(d);
+            if (OP::kCentred) centred += t[i] > 0.0f ? t[i] * d : 0.0f;
+        }
+        sum += sum_of<V>(t);
+    }
+    if (OP::kCentred) centred = team_sum<64>(centred);
+    RowStats s = join_waves<OP::kCentred, kPieceBlock / 64>(top, team_sum<64>((double)sum), centred);
+    if (threadIdx.x) return;
+    if (s.sum == 0.0) s.top = -INFINITY;  // nothing here: no maximum for the row's
+    w.parts[blockIdx.x] = s;
+    if (OP::kMoves && piece == 0) w.moves[row] = move_of<T>(r, op.moves, row);
+}
+
+// A block for every piece (for every row where an operator has no elements).
+template <typename T, typename OP>
+__global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
+    constexpr int V = Pack<T>::V, K = kPieceVectors;
+    const int64_t row = OP::kElements ? blockIdx.x / w.pieces : blockIdx.x;
+    const int piece = OP::kElements ? blockIdx.x % w.pieces : 0;
+    const RowStats *parts = w.parts + row * w.pieces;
+    // a thread's parts, then its wavefront's, then the block's
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < w.pieces; i += kPieceBlock) top = fmaxf(top, parts[i].top);
+    top = team_max<64>(top);
+    double sum = 0.0;
+    float centred = 0.0f;
+    for (int i = threadIdx.x; i < w.pieces; i += kPieceBlock) {
+        const bool empty = parts[i].top == -INFINITY;
+        const float d = empty ? 0.0f : parts[i].top - top, f = exp_of(d);
+        sum += parts[i].sum * (double)f;
+        if (OP::kCentred) centred += (parts[i].centred + (float)parts[i].sum * d) * f;
+    }
+    if (OP::kCentred) centred = team_sum<64>(centred);
+    const RowStats s = join_waves<OP::kCentred, kPieceBlock / 64>(top, team_sum<64>(sum), centred);
+    __shared__ RowOut shared_out;
+    if (threadIdx.x < 64) {
+        const Move m = OP::kMoves ? w.moves[row] : Move{-1, -INFINITY};
+        const RowOut o = op.row(row, s, m, piece == 0 && threadIdx.x == 0);
+        if (threadIdx.x == 0) {
+            shared_out = o;
+            if (OP::kLoss && piece == 0) op.block_loss[row] = o.share;
+        }
+    }
+    if constexpr (OP::kElements) {
+        __syncthreads();
+        typedef typename OP::template Element<T> OUT;
+        const RowOut out = shared_out;
+        OUT *to = op.template elements<OUT>(row);
+        if (!to) return;
+        const int head = head_of<T>(r, row), first = piece * (K * kPieceBlock) + threadIdx.x;
+        const int at = out.move < 0 ? -1 : out.move + head;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int vec = first + k * kPieceBlock, j = vec * V - head;
+            if (j >= r.actions) continue;
+            Pack<T> p;
+            uint32_t bits = inside_bits<V>(j, r.actions);
+            load_vector<T>(r, row, j, bits, p);
+            if (r.legal) bits &= legal_bits(r.legal + row * r.legal_stride, r.words, j);
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                y[i] = out.none || !(bits >> i & 1u) ? 0.0f : exp_of((float)p.x[i] - s.top) * out.each;
+            if (at >= 0 && at / V == vec) {
+#pragma unroll
+                for (int i = 0; i < V; i++) y[i] += at % V == i ? out.at_move : 0.0f;
+            }
+            store_vector<T, OUT>(to, op.aligned, j, r.actions, y);
+        }
+    }
+}
+
+// ---- the gradient of rows whose slope is known ----
+
+constexpr int kGradientVectors = 4;  // of a lane
+
+// A wavefront takes kGradientVectors * 64 vectors of a row.  Rows are taken from the last to the first: those that the
+// look at all rows has read last are in the cache still.
+template <typename T>
+__global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces) {
+    constexpr int V = Pack<T>::V, K = kGradientVectors;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), back = item / pieces;
+    if (back >= r.rows) return;
+    const int64_t row = r.rows - 1 - back;
+    const LineRows lines = line_rows(p, r.rows);
+    const bool rest = row < lines.begin || row >= lines.end;
+    if (rest && !p.zero_rest) return;
+    const float slope = rest ? 0.0f : p.slope[row], top = rest ? 0.0f : p.top[row];
+    const float each = rest ? 0.0f : -slope * p.inverse[row];
+    const int head = head_of<T>(r, row), first = (int)(item % pieces) * (K * 64) + lane;
+    const int at = slope == 0.0f ? -1 : p.moves[row] + head;
+    T *to = (T *)p.grad + row * p.grad_stride;
+    Pack<T> x[K];
+    uint32_t bits[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int j = (first + k * 64) * V - head;
+        bits[k] = slope == 0.0f ? 0u : inside_bits<V>(j, r.actions);
+        load_vector<T>(r, row, j, bits[k], x[k]);
+    }
+    if (r.legal) {
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (bits[k]) bits[k] &= legal_bits(r.legal + row * r.legal_stride, r.words, (first + k * 64) * V - head);
+    }
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int vec = first + k * 64, j = vec * V - head;
+        if (j >= r.actions) continue;
+        float y[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) y[i] = bits[k] >> i & 1u ? exp_of((float)x[k].x[i] - top) * each : 0.0f;
+        if (at >= 0 && at / V == vec) {
+#pragma unroll
+            for (int i = 0; i < V; i++) y[i] += at % V == i ? slope : 0.0f;
+        }
+        store_vector<T, T>(to, aligned, j, r.actions, y);
+    }
+}
+
+// ---- which kernel ----
+
+// Vectors of the widest row, whatever its head.
+template <typename T>
+static inline int64_t vectors_of(const Rows &r) {
+    constexpr int V = Pack<T>::V;
+    const int64_t most = r.actions + (r.aligned && r.rows > 1 && r.stride % V ? V - 1 : 0);
+    return (most + V - 1) / V;
+}
+
+// Blocks of a launch, which leave a share of the loss each (rows, where they are cut).
+struct Launched {
+    hipError_t error;
+    int64_t shares;
+};
+
+template <typename T, int TEAM, int K, typename OP>
+static Launched run_rows(const Rows &r, const OP &op, hipStream_t stream) {
+    constexpr int per_block = TEAM <= 64 ? 256 / TEAM : 1;
+    const int64_t blocks = (r.rows + per_block - 1) / per_block;
+    OP o = op;
+    if constexpr (OP::kLoss)
+        if (blocks == 1) o.block_loss = op.p.loss;  // its share is the loss
+    k_rows<T, TEAM, K, OP><<<(unsigned)blocks, TEAM <= 64 ? 256 : TEAM, 0, stream>>>(r, o);
+    return {hipGetLastError(), blocks};
+}
+
+// The narrowest team that holds a row.
+template <typename T, typename OP>
+static Launched run(const Rows &r, const OP &op, const Wide &w, hipStream_t stream) {
+    const int64_t n = vectors_of<T>(r);
+    if (n <= 32) return run_rows<T, 32, 1>(r, op, stream);
+    if (n <= 64) return run_rows<T, 64, 1>(r, op, stream);
+    if (n <= 128) return run_rows<T, 64, 2>(r, op, stream);
+    if (n <= 256) return run_rows<T, 64, 4>(r, op, stream);
+    if (n <= 512) return run_rows<T, 256, 2>(r, op, stream);
+    if (n <= 1024) return run_rows<T, 256, 4>(r, op, stream);
+    if (n <= 2048) return run_rows<T, 1024, 2>(r, op, stream);
+    if (n <= 4096) return run_rows<T, 1024, 4>(r, op, stream);
+    if (n <= 8192) return run_rows<T, 1024, 8>(r, op, stream);
+    if constexpr (sizeof(T) == 4)
+        if (n <= 16384) return run_rows<T, 1024, 16>(r, op, stream);
+    k_parts<T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, op, w);
+    k_apply<T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, op, w);
+    return {hipGetLastError(), r.rows};
+}
+
+// Work space of rows that are cut into pieces, at the end of what the caller gives (behind `before` bytes).
+template <typename T>
+static Wide wide_of(const Rows &r, void *work, int64_t before) {
+    Wide w = {(int32_t)((vectors_of<T>(r) + kPieceBlock * kPieceVectors - 1) / (kPieceBlock * kPieceVectors)), nullptr, nullptr};
+    w.parts = (RowStats *)((char *)work + (before + 15) / 16 * 16);
+    w.moves = (Move *)(w.parts + r.rows * w.pieces);
+    return w;
+}
+
+// Bases at multiples of 16 bytes and strides that agree in the vectors' lengths: then results have the logits' heads.
+template <typename T>
+static bool aligned_with(const Rows &r, const void *d, int64_t stride) {
+    return r.aligned && ((uintptr_t)d & 15) == 0 && (r.rows < 2 || (stride - r.stride) % Pack<T>::V == 0);
+}
+
+template <typename T>
+Launched type_priors(const Rows &r, float *priors, int64_t stride, void *work, hipStream_t stream) {
+    const PriorsOp op = {nullptr, nullptr, priors, stride, aligned_with<T>(r, priors, stride)};
+    return run<T>(r, op, wide_of<T>(r, work, 0), stream);
+}
+
+template <typename T>
+Launched type_logprobs(const Rows &r, const int32_t *moves, float *logprob, float *entropy, void *work, hipStream_t stream) {
+    const LogprobsOp op = {logprob ? moves : nullptr, nullptr, logprob, entropy};
+    return run<T>(r, op, wide_of<T>(r, work, 0), stream);
+}
+
+template <typename T>
+Launched type_policy_loss(const Rows &r, const PolicyLoss &p, hipStream_t stream) {
+    const PolicyOp op = {p.moves, p.shares, p, p.grad && aligned_with<T>(r, p.grad, p.grad_stride)};
+    return run<T>(r, op, wide_of<T>(r, p.shares, r.rows * 4), stream);
+}
+
+template <typename T>
+Launched type_lines(const Rows &r, const PreferenceLoss &p, int64_t before, hipStream_t stream) {
+    const LineOp op = {p.moves, nullptr, p};
+    return run<T>(r, op, wide_of<T>(r, p.work, before), stream);
+}
+
+template <typename T>
+hipError_t type_line_gradient(const Rows &r, const PreferenceLoss &p, hipStream_t stream) {
+    const int64_t pieces = (vectors_of<T>(r) + 64 * kGradientVectors - 1) / (64 * kGradientVectors);
+    k_line_gradient<T><<<(unsigned)((r.rows * pieces + 3) / 4), 256, 0, stream>>>(
+        r, p, aligned_with<T>(r, p.grad, p.grad_stride), (int)pieces);
+    return hipGetLastError();
+}
+
+#define OMK_POLICY_TYPE(WORD, T)                                                                                         \
+    WORD template Launched type_priors<T>(const Rows &, float *, int64_t, void *, hipStream_t);                          \
+    WORD template Launched type_logprobs<T>(const Rows &, const int32_t *, float *, float *, void *, hipStream_t);       \
+    WORD template Launched type_policy_loss<T>(const Rows &, const PolicyLoss &, hipStream_t);                           \
+    WORD template Launched type_lines<T>(const Rows &, const PreferenceLoss &, int64_t, hipStream_t);                    \
+    WORD template hipError_t type_line_gradient<T>(const Rows &, const PreferenceLoss &, hipStream_t);
+
+}  // namespace omk

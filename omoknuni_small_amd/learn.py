@@ -16,7 +16,7 @@ from .forest import _check, load_library
 
 EXPORTS = [
     "omk_learner_create", "omk_learner_destroy", "omk_learner_set_stream", "omk_learner_get_stream", "omk_learner_sync",
-    "omk_policy_priors", "omk_policy_logprobs", "omk_policy_loss_work", "omk_policy_loss",
+    "omk_policy_work", "omk_policy_priors", "omk_policy_logprobs", "omk_policy_loss_work", "omk_policy_loss",
     "omk_preference_loss_work", "omk_preference_loss",
     "omk_adamw_create", "omk_adamw_destroy", "omk_adamw_step", "omk_adamw_set_steps", "omk_adamw_get_steps",
 ]
@@ -65,7 +65,8 @@ class _AdamDesc(C.Structure):
 _ARGTYPES = {
     "omk_learner_create": (_I32, _VP), "omk_learner_destroy": (_VP,), "omk_learner_set_stream": (_VP, _VP),
     "omk_learner_get_stream": (_VP, _VP), "omk_learner_sync": (_VP,),
-    "omk_policy_priors": (_VP, _VP, _VP, _I64), "omk_policy_logprobs": (_VP, _VP, _VP, _VP, _VP),
+    "omk_policy_work": (_I64, _I32), "omk_policy_priors": (_VP, _VP, _VP, _I64, _VP, _I64),
+    "omk_policy_logprobs": (_VP, _VP, _VP, _VP, _VP, _VP, _I64),
     "omk_policy_loss_work": (_I64, _I32), "omk_policy_loss": (_VP, _VP, _VP, _VP, _VP, _VP, _I64),
     "omk_preference_loss_work": (_I64, _I32, _I64),
     "omk_preference_loss": (_VP, _VP, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _I64),
@@ -218,6 +219,11 @@ class Learner:
             raise ValueError("grad of shape %s, logits of %s" % (tuple(grad.shape), tuple(logits.shape)))
         return grad
 
+    def _work(self, need, logits):
+        if not need:
+            return None, 0
+        return _torch().empty(need, dtype=_torch().uint8, device=logits.device), need
+
     # ---- operators ----
 
     def priors(self, logits, legal=None, out=None):
@@ -231,21 +237,23 @@ class Learner:
             self._same_place("out", out, torch.float32)
             if tuple(out.shape) != (rows, actions) or (actions > 1 and out.stride(1) != 1):
                 raise ValueError("out of shape %s: [%d, %d] is wanted" % (tuple(out.shape), rows, actions))
+        work, need = self._work(self._lib.omk_policy_work(rows, actions), logits)
         self._on_stream()
-        _check(self._lib.omk_policy_priors(self._h, C.byref(r), out.data_ptr(), out.stride(0)))
+        _check(self._lib.omk_policy_priors(self._h, C.byref(r), out.data_ptr(), out.stride(0), None if work is None else work.data_ptr(), need))
         return out
 
     def logprobs(self, logits, moves=None, legal=None, entropy=False):
         """Logprobs(logprob, entropy), float32 [rows] each: the log-probability of the moves (None without moves; 0 for
         a move outside the action space, -inf for one that is not legal) and, if wanted, the entropy of the rows."""
         torch = _torch()
-        r, rows, _ = self._rows(logits, legal)
+        r, rows, actions = self._rows(logits, legal)
         d_moves = self._vector("moves", moves, rows, torch.int32)
         lp = None if moves is None else torch.empty(rows, dtype=torch.float32, device=logits.device)
         ent = torch.empty(rows, dtype=torch.float32, device=logits.device) if entropy else None
+        work, need = self._work(self._lib.omk_policy_work(rows, actions), logits)
         self._on_stream()
         _check(self._lib.omk_policy_logprobs(self._h, C.byref(r), d_moves, None if lp is None else lp.data_ptr(),
-                                             None if ent is None else ent.data_ptr()))
+                                             None if ent is None else ent.data_ptr(), None if work is None else work.data_ptr(), need))
         return Logprobs(lp, ent)
 
     def policy_loss(self, logits, moves, old_logprob, advantage, ref_logprob=None, weight=None, legal=None, clip_low=0.2,
@@ -265,13 +273,14 @@ class Learner:
         g = self._gradient(grad, logits)
         need = self._lib.omk_policy_loss_work(rows, actions)
         # one allocation for what is small: log-probabilities, kl, the loss, and the work space behind them
-        small = torch.empty(2 * rows + 1 + (need + 3) // 4, dtype=f32, device=logits.device)
+        behind = (2 * rows + 4) // 4 * 4
+        small = torch.empty(behind + (need + 3) // 4, dtype=f32, device=logits.device)
         at = small.data_ptr()
         out = _PolicyOut(at + 8 * rows, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                          at + 4 * rows)
         self._on_stream()
         _check(self._lib.omk_policy_loss(self._h, C.byref(r), C.byref(samples), C.byref(params), C.byref(out),
-                                         at + 8 * rows + 4, need))
+                                         at + 4 * behind, need))
         return PolicyLoss(small[2 * rows], g, small[:rows], small[rows:2 * rows])
 
     def preference_loss(self, logits, moves, line_begin, ref_logprob=None, legal=None, beta=0.1, label_smoothing=0.0,
@@ -295,13 +304,14 @@ class Learner:
         params = _PreferenceParams(beta, label_smoothing, 1.0 / max(pairs, 1) if scale is None else scale)
         g = self._gradient(grad, logits)
         need = self._lib.omk_preference_loss_work(rows, actions, pairs)
-        small = torch.empty(3 * pairs + 1 + (need + 3) // 4, dtype=f32, device=logits.device)
+        behind = (3 * pairs + 4) // 4 * 4
+        small = torch.empty(behind + (need + 3) // 4, dtype=f32, device=logits.device)
         at = small.data_ptr()
         out = _PreferenceOut(at + 12 * pairs, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                              at + 4 * pairs, grad is True)
         self._on_stream()
         _check(self._lib.omk_preference_loss(self._h, C.byref(r), d_moves, d_begin, pairs, d_ref, C.byref(params),
-                                             C.byref(out), at + 12 * pairs + 4, need))
+                                             C.byref(out), at + 4 * behind, need))
         return PreferenceLoss(small[3 * pairs], g, small[:pairs], small[pairs:3 * pairs])
 
 

@@ -92,7 +92,9 @@ def policy_loss(rows, moves, old, advantage, ref, weight, clip_low, clip_high, k
         d = np.where(counts, ref - lp, 0.0)
         kl = np.expm1(d) - d
         d_off = off + np.abs(d) * U
-        kl_off = np.abs(np.expm1(d)) * d_off + kl * 12 * U + (np.abs(np.expm1(d)) + np.abs(d)) * 4 * U * (np.abs(d) >= 0.25)
+        # exp(d + t) - (d + t) - 1 is (exp(d) - d - 1) + (exp(d) - 1) t + exp(d) t^2 / 2 + .., |t| <= d_off: where d is 0 the
+        # second term is all there is
+        kl_off = np.abs(np.expm1(d)) * d_off + np.exp(np.abs(d)) * d_off ** 2 + kl * 12 * U + (np.abs(np.expm1(d)) + np.abs(d)) * 4 * U * (np.abs(d) >= 0.25)
         row, row_off = row + kl_weight * kl, row_off + kl_weight * (kl_off + 3 * U * kl)
         slope = slope - kl_weight * np.expm1(d)
         slope_off = slope_off + kl_weight * (np.exp(d) * d_off + 6 * U * np.abs(np.expm1(d)))

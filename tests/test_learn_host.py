@@ -60,9 +60,9 @@ def test_rows_are_refused(handle, change):
     params = learn._PolicyParams(0.2, 0.2, 0.1, 1.0)
     pout = learn._PreferenceOut(address(2), address(3), 225, None, None, 0)
     pparams = learn._PreferenceParams(0.1, 0.0, 1.0)
-    assert lib.omk_policy_priors(handle, C.byref(r), address(3), 225) == INVALID
+    assert lib.omk_policy_priors(handle, C.byref(r), address(3), 225, None, 0) == INVALID
     assert message().startswith("omk_policy_priors: ")
-    assert lib.omk_policy_logprobs(handle, C.byref(r), address(5), address(2), None) == INVALID
+    assert lib.omk_policy_logprobs(handle, C.byref(r), address(5), address(2), None, None, 0) == INVALID
     assert lib.omk_policy_loss(handle, C.byref(r), C.byref(samples), C.byref(params), C.byref(out), address(11), 1 << 20) == INVALID
     assert lib.omk_preference_loss(handle, C.byref(r), address(5), address(6), 2, None, C.byref(pparams), C.byref(pout),
                                    address(11), 1 << 20) == INVALID
@@ -95,14 +95,26 @@ def test_policy_loss_refuses(handle):
     assert needed > 0
     assert policy(handle, work=needed - 1) == CAPACITY
     assert policy(handle, d_work=None) == CAPACITY
-    assert policy(handle, d_work=address(11) + 2) == INVALID
+    assert policy(handle, d_work=address(11) + 8) == INVALID
     assert policy(None) == INVALID
 
 
 def test_priors_may_not_lie_across_the_logits(handle):
     lib, r = learn._library(), rows(type=0)
     for at in (address(0), address(0) + 4 * 225 * 8 - 4, address(0) - 4 * 225 * 8 + 4):
-        assert lib.omk_policy_priors(handle, C.byref(r), at, 225) == INVALID and "across" in message()
+        assert lib.omk_policy_priors(handle, C.byref(r), at, 225, None, 0) == INVALID and "across" in message()
+
+
+def test_wide_rows_need_work_space(handle):
+    lib = learn._library()
+    assert lib.omk_policy_work(100, 65528) == 0 and lib.omk_policy_work(0, 1 << 20) == 0
+    needed = lib.omk_policy_work(8, 100000)
+    assert needed > 0
+    r = rows(actions=100000, row_stride=100000, d_legal=None)
+    for d_work, n in ((None, needed), (address(11), needed - 1)):
+        assert lib.omk_policy_priors(handle, C.byref(r), address(3), 100000, d_work, n) == CAPACITY
+        assert lib.omk_policy_logprobs(handle, C.byref(r), address(5), address(2), None, d_work, n) == CAPACITY
+    assert lib.omk_policy_priors(handle, C.byref(r), address(3), 100000, address(11) + 4, needed) == INVALID
 
 
 def preference(handle, params=(), out=(), pairs=3, work=1 << 20, d_moves=address(5), d_begin=address(6), d_work=address(11)):
