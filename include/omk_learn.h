@@ -161,7 +161,8 @@ typedef struct omk_adamw_desc {
     int32_t grad_type;  /* OMK_F32, or param_type, or with 32-bit parameters either 16-bit type */
     int32_t copy_type;  /* OMK_NONE, or with 32-bit parameters OMK_BF16 or OMK_F16 */
     int32_t state_type; /* OMK_F32, OMK_F8 */
-    double beta1, beta2, eps;
+    double beta1, beta2;
+    double eps; /* 0, or 2^-126 and more */
     uint32_t seed;
 } omk_adamw_desc;
 /* Copies the description to the device; the tensors stay the caller's, and where they are.  Pointers need the alignment of

@@ -357,8 +357,8 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     if (pt != OMK_F32 && ct != OMK_NONE)
         return learn_fail(OMK_ERR_UNSUPPORTED, "%s: a copy is kept of 32-bit parameters only", who);
     if (!(desc->beta1 >= 0.0 && desc->beta1 < 1.0) || !(desc->beta2 >= 0.0 && desc->beta2 < 1.0) || !(desc->eps >= 0.0) ||
-        !std::isfinite(desc->eps))
-        return learn_fail(OMK_ERR_INVALID, "%s: betas %g and %g (0 <= beta < 1), eps %g", who, desc->beta1, desc->beta2,
+        !((float)desc->eps <= 3e38f) || (desc->eps > 0.0 && desc->eps < 0x1p-126))
+        return learn_fail(OMK_ERR_INVALID, "%s: betas %g and %g (0 <= beta < 1), eps %g (0 or at least 2^-126)", who, desc->beta1, desc->beta2,
                           desc->eps);
     std::vector<AdamTensor> tensors((size_t)desc->n_tensors);
     std::vector<int64_t> first_chunk((size_t)desc->n_tensors + 1, 0), elements((size_t)desc->n_tensors);
@@ -378,7 +378,9 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
             return learn_fail(OMK_ERR_INVALID, "%s: tensor %d: an address that is no multiple of its type's size", who, i);
         const int64_t own = (t.n + kUnit - 1) / kUnit;
         tensors[i] = AdamTensor{t.n, t.d_param, t.d_copy, t.d_m, t.d_v, t.d_m_scale, t.d_v_scale, units,
-                                (float)t.lr_scale, (float)t.weight_decay};
+                                (float)t.lr_scale, (float)t.weight_decay,
+                                aligned(t.d_param, 4 * width_of(pt)) && aligned(t.d_copy, 8) &&
+                                    aligned(t.d_m, 4 * width_of(st)) && aligned(t.d_v, 4 * width_of(st))};
         elements[i] = t.n;
         first_chunk[i] = n_chunks;
         units += own;
@@ -419,7 +421,7 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     }
     if (e == hipSuccess && !chunks.empty())
         e = hipMemcpy(o->chunks, chunks.data(), chunks.size() * sizeof(AdamChunk), hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = launch_adamw_set(o->count, 0, 1.0, 1.0, l->stream);
+    if (e == hipSuccess) e = launch_adamw_set(o->count, 0, o->beta1, o->beta2, l->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(l->stream);
     if (e != hipSuccess) {
         const int rc = learn_fail(OMK_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
@@ -445,6 +447,7 @@ int omk_adamw_step(omk_adamw *o, const void *const *h_grads, double lr, const fl
     AdamStep s;
     s.tensors = o->tensors;
     s.count = o->count;
+    s.chunk_units = kChunkUnits;
     s.d_lr = d_lr;
     s.d_grad_scale = d_grad_scale;
     s.lr = lr;
@@ -472,7 +475,7 @@ int omk_adamw_set_steps(omk_adamw *o, int64_t steps) {
     if (steps < 0 || steps > INT32_MAX) return learn_fail(OMK_ERR_INVALID, "%s: %lld steps", who, (long long)steps);
     OnDevice on(o->l->device);
     LEARN_TRY(on.status);
-    LEARN_TRY(launch_adamw_set(o->count, steps, std::pow(o->beta1, (double)steps), std::pow(o->beta2, (double)steps),
+    LEARN_TRY(launch_adamw_set(o->count, steps, std::pow(o->beta1, (double)steps + 1.0), std::pow(o->beta2, (double)steps + 1.0),
                                o->l->stream));
     return OMK_OK;
 }

@@ -66,7 +66,7 @@ hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss 
 hipError_t launch_set_float(float *to, float value, hipStream_t stream);
 
 constexpr int kUnit = 256;      // elements that share a scale, and that a wavefront steps at a time
-constexpr int kChunkUnits = 8;  // units of a chunk: what a block takes at a time, all of one tensor
+constexpr int kChunkUnits = 32;  // units of a chunk: what a block takes at a time, all of one tensor
 constexpr int kGradsPerLaunch = 256;  // gradient pointers that travel as kernel arguments
 
 struct AdamTensor {
@@ -75,6 +75,7 @@ struct AdamTensor {
     float *m_scale, *v_scale;
     int64_t first_unit;  // units of the tensors before it
     float lr_scale, weight_decay;
+    bool vectors;  // all addresses (but the gradient's) are multiples of four elements
 };
 
 struct AdamChunk {
@@ -82,11 +83,13 @@ struct AdamChunk {
     int32_t chunk;  // of the tensor's
 };
 
-// Lives on the device: steps done, beta1^steps, beta2^steps, and the blocks of the running step that are done.
+// Lives on the device: steps done, and what the next step, t, is made with: beta1^t, beta2^t, 1 / (1 - beta1^t) and
+// 1 / sqrt(1 - beta2^t), which every block would have to work out; and the blocks of that step that are done.
 struct AdamCount {
-    double power1, power2;
+    double power1, power2, unbias;
+    float root;
+    uint32_t done;
     int64_t steps;
-    uint32_t done, reserved;
 };
 
 struct AdamGrads {
@@ -97,6 +100,7 @@ struct AdamStep {
     const AdamTensor *tensors;
     const AdamChunk *chunks;
     int64_t n_chunks;
+    int32_t chunk_units;
     int32_t first_tensor;
     AdamCount *count;
     const float *d_lr, *d_grad_scale;

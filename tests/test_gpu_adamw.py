@@ -86,9 +86,10 @@ class Plain:
                 update = rate * m.astype(np.float64) / down
             shrink = lr * self.lr_scale[i] * self.decay[i]
             new = p[i] * (1 - shrink) - update
-            # a rounded rate, its product, the root's (half a step and a rounded factor), a sum, a quotient: 8 U of the
-            # update; the decay's product and both differences: 2 U of what they give
-            off = np.abs(update) * 8 * U + np.abs(p[i] * shrink) * 3 * U + (np.abs(p[i]) + np.abs(new)) * 2 * U
+            # a rounded rate and its product (2 U), the root's half step, a rounded factor and its product (3 U), a sum (U),
+            # a reciprocal that is good to a step (2 U) and its product (U): 9 U of the update; the decay's product and
+            # both differences: 2 U of what they give
+            off = np.abs(update) * 9 * U + np.abs(p[i] * shrink) * 3 * U + (np.abs(p[i]) + np.abs(new)) * 2 * U
             out.append((new, off))
             self.m[i], self.v[i] = m, v
             if self.states == "f8":

@@ -164,7 +164,7 @@ def test_adamw_refuses(handle):
         assert adamw(handle, tensor=change) == INVALID, change
     for change in (dict(n_tensors=-1), dict(h_tensors=None), dict(param_type=3), dict(grad_type=-1), dict(copy_type=0),
                    dict(copy_type=3), dict(state_type=1), dict(state_type=-1), dict(beta1=1.0), dict(beta1=-0.1),
-                   dict(beta2=math.nan), dict(eps=-1.0), dict(eps=math.nan), dict(copy_type=1)):
+                   dict(beta2=math.nan), dict(eps=-1.0), dict(eps=math.nan), dict(eps=1e-40), dict(eps=1e39), dict(copy_type=1)):
         assert adamw(handle, **change) == INVALID, change
     for change in (dict(d_m_scale=None), dict(d_v_scale=None), dict(d_v_scale=address(4) + 2)):
         assert adamw(handle, tensor=change, state_type=3) == INVALID, change
