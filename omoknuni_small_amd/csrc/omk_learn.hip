@@ -25,7 +25,9 @@ struct omk_adamw {
     int32_t param_type = 0, grad_type = 0, copy_type = 0, state_type = 0;
     double beta1 = 0, beta2 = 0, eps = 0;
     uint32_t seed = 0;
-    char *memory = nullptr;  // the count, the tensors, the chunks
+    int32_t chunk_units = 0;
+    char *memory = nullptr;  // the count and its groups' counters, the tensors, the chunks
+    uint32_t *done = nullptr;
     AdamCount *count = nullptr;
     AdamTensor *tensors = nullptr;
     AdamChunk *chunks = nullptr;
@@ -363,6 +365,10 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     std::vector<AdamTensor> tensors((size_t)desc->n_tensors);
     std::vector<int64_t> first_chunk((size_t)desc->n_tensors + 1, 0), elements((size_t)desc->n_tensors);
     int64_t units = 0, n_chunks = 0;
+    for (int32_t i = 0; i < desc->n_tensors; i++)
+        units += std::max((int64_t)0, std::min(desc->h_tensors[i].n, (int64_t)1 << 40) / kUnit);
+    const int32_t chunk_units = units < kManyUnits ? kFewUnits : kChunkUnits;
+    units = 0;
     for (int32_t i = 0; i < desc->n_tensors; i++) {
         const omk_adamw_tensor &t = desc->h_tensors[i];
         if (t.n < 0 || t.n > (int64_t)1 << 40) return learn_fail(OMK_ERR_INVALID, "%s: tensor %d of %lld elements", who, i, (long long)t.n);
@@ -384,7 +390,7 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
         elements[i] = t.n;
         first_chunk[i] = n_chunks;
         units += own;
-        n_chunks += (own + kChunkUnits - 1) / kChunkUnits;
+        n_chunks += (own + chunk_units - 1) / chunk_units;
     }
     first_chunk[(size_t)desc->n_tensors] = n_chunks;
     if (units > UINT32_MAX || n_chunks > INT32_MAX)
@@ -406,14 +412,16 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     o->beta2 = desc->beta2;
     o->eps = desc->eps;
     o->seed = desc->seed;
+    o->chunk_units = chunk_units;
     o->first_chunk.swap(first_chunk);
     o->elements.swap(elements);
     OnDevice on(l->device);
-    const size_t at_tensors = 256, at_chunks = at_tensors + (tensors.size() * sizeof(AdamTensor) + 255) / 256 * 256;
+    const size_t at_done = 256, at_tensors = at_done + kCountGroups * kCountStep * 4, at_chunks = at_tensors + (tensors.size() * sizeof(AdamTensor) + 255) / 256 * 256;
     hipError_t e = on.status;
     if (e == hipSuccess) e = hipMalloc((void **)&o->memory, at_chunks + chunks.size() * sizeof(AdamChunk) + 16);
     if (e == hipSuccess) {
         o->count = (AdamCount *)o->memory;
+        o->done = (uint32_t *)(o->memory + at_done);
         o->tensors = (AdamTensor *)(o->memory + at_tensors);
         o->chunks = (AdamChunk *)(o->memory + at_chunks);
         if (!tensors.empty())
@@ -421,7 +429,7 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     }
     if (e == hipSuccess && !chunks.empty())
         e = hipMemcpy(o->chunks, chunks.data(), chunks.size() * sizeof(AdamChunk), hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = launch_adamw_set(o->count, 0, o->beta1, o->beta2, l->stream);
+    if (e == hipSuccess) e = launch_adamw_set(o->count, o->done, 0, o->beta1, o->beta2, l->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(l->stream);
     if (e != hipSuccess) {
         const int rc = learn_fail(OMK_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
@@ -447,7 +455,8 @@ int omk_adamw_step(omk_adamw *o, const void *const *h_grads, double lr, const fl
     AdamStep s;
     s.tensors = o->tensors;
     s.count = o->count;
-    s.chunk_units = kChunkUnits;
+    s.done = o->done;
+    s.chunk_units = o->chunk_units;
     s.d_lr = d_lr;
     s.d_grad_scale = d_grad_scale;
     s.lr = lr;
@@ -475,7 +484,7 @@ int omk_adamw_set_steps(omk_adamw *o, int64_t steps) {
     if (steps < 0 || steps > INT32_MAX) return learn_fail(OMK_ERR_INVALID, "%s: %lld steps", who, (long long)steps);
     OnDevice on(o->l->device);
     LEARN_TRY(on.status);
-    LEARN_TRY(launch_adamw_set(o->count, steps, std::pow(o->beta1, (double)steps + 1.0), std::pow(o->beta2, (double)steps + 1.0),
+    LEARN_TRY(launch_adamw_set(o->count, o->done, steps, std::pow(o->beta1, (double)steps + 1.0), std::pow(o->beta2, (double)steps + 1.0),
                                o->l->stream));
     return OMK_OK;
 }

@@ -66,7 +66,10 @@ hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss 
 hipError_t launch_set_float(float *to, float value, hipStream_t stream);
 
 constexpr int kUnit = 256;      // elements that share a scale, and that a wavefront steps at a time
-constexpr int kChunkUnits = 32;  // units of a chunk: what a block takes at a time, all of one tensor
+// Units of a chunk: what a block takes at a time, all of one tensor.  kChunkUnits where there are enough of them to
+// fill the card with blocks, kFewUnits (a unit a wavefront) in smaller networks.
+constexpr int kChunkUnits = 32, kFewUnits = 4;
+constexpr int64_t kManyUnits = 16384;
 constexpr int kGradsPerLaunch = 256;  // gradient pointers that travel as kernel arguments
 
 struct AdamTensor {
@@ -84,13 +87,15 @@ struct AdamChunk {
 };
 
 // Lives on the device: steps done, and what the next step, t, is made with: beta1^t, beta2^t, 1 / (1 - beta1^t) and
-// 1 / sqrt(1 - beta2^t), which every block would have to work out; and the blocks of that step that are done.
+// 1 / sqrt(1 - beta2^t), which every block would have to work out; and the groups of blocks that are done with that step.
 struct AdamCount {
     double power1, power2, unbias;
     float root;
     uint32_t done;
     int64_t steps;
 };
+
+constexpr int kCountGroups = 64, kCountStep = 32;  // counters of blocks that are done, 128 bytes apart
 
 struct AdamGrads {
     const void *g[kGradsPerLaunch];
@@ -103,6 +108,7 @@ struct AdamStep {
     int32_t chunk_units;
     int32_t first_tensor;
     AdamCount *count;
+    uint32_t *done;  // the groups' counters, 0 between steps
     const float *d_lr, *d_grad_scale;
     double lr;
     double beta1, beta2;
@@ -113,6 +119,6 @@ struct AdamStep {
 
 hipError_t launch_adamw(int param, int grad, int copy, int state, const AdamStep &s, const AdamGrads &g,
                         hipStream_t stream);
-hipError_t launch_adamw_set(AdamCount *count, int64_t steps, double power1, double power2, hipStream_t stream);
+hipError_t launch_adamw_set(AdamCount *count, uint32_t *done, int64_t steps, double power1, double power2, hipStream_t stream);
 
 }  // namespace omk
