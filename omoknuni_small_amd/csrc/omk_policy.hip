@@ -9,18 +9,9 @@ OMK_POLICY_TYPE(extern, f16_t)
 
 constexpr int kSumBlock = 1024;
 
-// The sum of n values, in one order whatever runs beside it.
 __global__ __launch_bounds__(kSumBlock) void k_sum(const float *values, int64_t n, float *out) {
-    __shared__ double part[kSumBlock / 64];
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kSumBlock) s += (double)values[i];
-    s = team_sum<64>(s);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x) return;
-    s = 0.0;
-    for (int i = 0; i < kSumBlock / 64; i++) s += part[i];
-    *out = (float)s;
+    const double s = block_sum<kSumBlock>(values, n);
+    if (threadIdx.x == 0) *out = (float)s;
 }
 
 // A wavefront for every pair of lines: the lines' sums, the pair's loss, and the slope of every row of theirs.
@@ -117,10 +108,14 @@ hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss 
         if (l.error != hipSuccess) return l.error;
     }
     k_pairs<<<(unsigned)((p.pairs + 3) / 4), 256, 0, stream>>>(r, p);
-    k_sum<<<1, kSumBlock, 0, stream>>>(p.pair_loss, p.pairs, p.loss);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && p.grad) OMK_BY_TYPE(type, e = type_line_gradient<T>(r, p, stream));
-    return e;
+    if (e != hipSuccess) return e;
+    if (p.grad) {
+        OMK_BY_TYPE(type, e = type_line_gradient<T>(r, p, stream));
+        return e;
+    }
+    k_sum<<<1, kSumBlock, 0, stream>>>(p.pair_loss, p.pairs, p.loss);
+    return hipGetLastError();
 }
 
 }  // namespace omk

@@ -512,12 +512,36 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
 
 constexpr int kGradientVectors = 4;  // of a lane
 
-// A wavefront takes kGradientVectors * 64 vectors of a row.  Rows are taken from the last to the first: those that the
+// The sum of n values by one block, in one order whatever runs beside it: in its first thread.
+template <int BLOCK>
+__device__ __forceinline__ double block_sum(const float *values, int64_t n) {
+    __shared__ double part[BLOCK / 64];
+    double s = 0.0;
+    // (four at a time, so that as many loads are on their way)
+    int64_t i = threadIdx.x;
+    for (; i + 3 * BLOCK < n; i += 4 * BLOCK) {
+        const float a = values[i], b = values[i + BLOCK], c = values[i + 2 * BLOCK], d = values[i + 3 * BLOCK];
+        s += ((double)a + (double)b) + ((double)c + (double)d);
+    }
+    for (; i < n; i += BLOCK) s += (double)values[i];
+    s = team_sum<64>(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0;
+    for (int w = 0; w < BLOCK / 64; w++) s += part[w];
+    return s;
+}
+
+// A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.  Rows are taken from the last to the first: those that the
 // look at all rows has read last are in the cache still.
 template <typename T>
 __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces) {
     constexpr int V = Pack<T>::V, K = kGradientVectors;
     const int lane = threadIdx.x & 63;
+    if (blockIdx.x == 0) {
+        const double loss = block_sum<256>(p.pair_loss, p.pairs);
+        if (threadIdx.x == 0) *p.loss = (float)loss;
+    }
     const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), back = item / pieces;
     if (back >= r.rows) return;
     const int64_t row = r.rows - 1 - back;

@@ -132,21 +132,30 @@ class Learner:
     """A device, and the operators on rows of logits there (omk_learner).
 
     Rows are positions (or tokens) and columns actions: logits [rows, actions] in float32, bfloat16 or float16 with any
-    stride between rows.  `legal`: int32 masks [rows, words], or [words] for all rows alike, as pack_legal makes them (None: all
-    actions are legal).  `moves`: int32 [rows], -1 where a row is padding.  See include/omk_learn.h for rows without a
-    legal action and for infinite logits.
+    stride between rows.  `legal`: int32 masks [rows, words], or [words] for all rows alike, as pack_legal makes them (None:
+    all actions are legal).  `moves`: int32 [rows], -1 where a row is padding.  See include/omk_learn.h for rows without
+    a legal action and for infinite logits.
     """
 
     def __init__(self, device=None):
         self._lib = _library()
         self._h = C.c_void_p()
-        if device is None or not isinstance(device, int):
-            torch = _torch()
-            device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+        import torch
+        self._torch = torch
+        if device is None:
+            device = torch.cuda.current_device()
+        elif not isinstance(device, int):
+            device = torch.device(device)
+            device = torch.cuda.current_device() if device.index is None else device.index
         self.device = int(device)
         _check(self._lib.omk_learner_create(self.device, C.byref(self._h)))
         self._stream = 0
         self._types = _types()
+        self._empty, self._f32, self._i32 = torch.empty, torch.float32, torch.int32
+        self._place = torch.device("cuda", self.device)
+        # (the address alone: the stream object of torch.cuda.current_stream costs a microsecond)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def close(self):
         if self._h:
@@ -166,52 +175,51 @@ class Learner:
     # ---- arguments ----
 
     def _on_stream(self):
-        stream = _torch().cuda.current_stream(self.device).cuda_stream
+        stream = self._raw_stream(self.device)
         if stream != self._stream:
             _check(self._lib.omk_learner_set_stream(self._h, stream))
             self._stream = stream
 
     def _rows(self, logits, legal):
-        torch = _torch()
         kind = self._types.get(logits.dtype)
         if kind is None:
             raise TypeError("logits of %s: float32, bfloat16 or float16 are taken" % logits.dtype)
         if logits.dim() != 2 or logits.shape[1] < 1:
             raise ValueError("logits of shape %s: [rows, actions] is wanted" % (tuple(logits.shape),))
-        if not logits.is_cuda or logits.device.index != self.device:
+        if logits.get_device() != self.device:
             raise ValueError("logits on %s: the learner's device is %d" % (logits.device, self.device))
         rows, actions = logits.shape
-        if actions > 1 and logits.stride(1) != 1:
-            raise ValueError("logits whose actions are %d elements apart" % logits.stride(1))
-        r = _Rows(logits.data_ptr(), logits.stride(0), rows, actions, kind, None, 0)
-        if legal is not None:
-            words = (actions + 31) // 32
-            self._same_place("legal", legal, torch.int32)
-            if tuple(legal.shape) not in ((rows, words), (words,)):
-                raise ValueError("legal of shape %s: [%d, %d] or [%d] is wanted" % (tuple(legal.shape), rows, words, words))
-            if words > 1 and legal.stride(-1) != 1:
-                raise ValueError("legal whose words are %d apart" % legal.stride(-1))
-            r.d_legal = legal.data_ptr()
-            r.legal_stride = 0 if legal.dim() == 1 else legal.stride(0)
-        return r, rows, actions
+        stride, step = logits.stride()
+        if step != 1 and actions > 1:
+            raise ValueError("logits whose actions are %d elements apart" % step)
+        if legal is None:
+            return _Rows(logits.data_ptr(), stride, rows, actions, kind, None, 0), rows, actions
+        words = (actions + 31) // 32
+        self._same_place("legal", legal, self._i32)
+        if tuple(legal.shape) not in ((rows, words), (words,)):
+            raise ValueError("legal of shape %s: [%d, %d] or [%d] is wanted" % (tuple(legal.shape), rows, words, words))
+        if words > 1 and legal.stride(-1) != 1:
+            raise ValueError("legal whose words are %d apart" % legal.stride(-1))
+        return _Rows(logits.data_ptr(), stride, rows, actions, kind, legal.data_ptr(),
+                     0 if legal.dim() == 1 else legal.stride(0)), rows, actions
 
     def _same_place(self, name, x, dtype):
         if x.dtype != dtype:
             raise TypeError("%s of %s: %s is wanted" % (name, x.dtype, dtype))
-        if not x.is_cuda or x.device.index != self.device:
+        if x.get_device() != self.device:
             raise ValueError("%s on %s: the learner's device is %d" % (name, x.device, self.device))
 
     def _vector(self, name, x, n, dtype):
         if x is None:
             return None
+        if x.dtype is dtype and x.get_device() == self.device and x.dim() == 1 and x.numel() == n and x.is_contiguous():
+            return x.data_ptr()
         self._same_place(name, x, dtype)
-        if x.dim() != 1 or x.shape[0] != n or (n > 1 and x.stride(0) != 1):
-            raise ValueError("%s of shape %s: %d values in a row are wanted" % (name, tuple(x.shape), n))
-        return x.data_ptr()
+        raise ValueError("%s of shape %s: %d values in a row are wanted" % (name, tuple(x.shape), n))
 
     def _gradient(self, grad, logits):
         if grad is True:
-            return _torch().empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            return self._empty(logits.shape, dtype=logits.dtype, device=self._place)
         if grad is None or grad is False:
             return None
         self._same_place("grad", grad, logits.dtype)
@@ -219,41 +227,42 @@ class Learner:
             raise ValueError("grad of shape %s, logits of %s" % (tuple(grad.shape), tuple(logits.shape)))
         return grad
 
-    def _work(self, need, logits):
-        if not need:
-            return None, 0
-        return _torch().empty(need, dtype=_torch().uint8, device=logits.device), need
+    def _work(self, rows, actions):
+        """Work space of the calls that need some for wide rows only."""
+        need = self._lib.omk_policy_work(rows, actions)
+        return (self._empty(need, dtype=self._torch.uint8, device=self._place), need) if need else (None, 0)
 
     # ---- operators ----
 
     def priors(self, logits, legal=None, out=None):
         """Probabilities of the actions, float32 [rows, actions]: 0 where an action is not legal, and in a row that has
         no legal action."""
-        torch = _torch()
         r, rows, actions = self._rows(logits, legal)
         if out is None:
-            out = torch.empty((rows, actions), dtype=torch.float32, device=logits.device)
+            out, stride = self._empty((rows, actions), dtype=self._f32, device=self._place), actions
         else:
-            self._same_place("out", out, torch.float32)
+            self._same_place("out", out, self._f32)
             if tuple(out.shape) != (rows, actions) or (actions > 1 and out.stride(1) != 1):
                 raise ValueError("out of shape %s: [%d, %d] is wanted" % (tuple(out.shape), rows, actions))
-        work, need = self._work(self._lib.omk_policy_work(rows, actions), logits)
+            stride = out.stride(0)
+        work, need = self._work(rows, actions)
         self._on_stream()
-        _check(self._lib.omk_policy_priors(self._h, C.byref(r), out.data_ptr(), out.stride(0), None if work is None else work.data_ptr(), need))
+        _check(self._lib.omk_policy_priors(self._h, C.byref(r), out.data_ptr(), stride,
+                                           None if work is None else work.data_ptr(), need))
         return out
 
     def logprobs(self, logits, moves=None, legal=None, entropy=False):
         """Logprobs(logprob, entropy), float32 [rows] each: the log-probability of the moves (None without moves; 0 for
         a move outside the action space, -inf for one that is not legal) and, if wanted, the entropy of the rows."""
-        torch = _torch()
         r, rows, actions = self._rows(logits, legal)
-        d_moves = self._vector("moves", moves, rows, torch.int32)
-        lp = None if moves is None else torch.empty(rows, dtype=torch.float32, device=logits.device)
-        ent = torch.empty(rows, dtype=torch.float32, device=logits.device) if entropy else None
-        work, need = self._work(self._lib.omk_policy_work(rows, actions), logits)
+        d_moves = self._vector("moves", moves, rows, self._i32)
+        lp = None if moves is None else self._empty(rows, dtype=self._f32, device=self._place)
+        ent = self._empty(rows, dtype=self._f32, device=self._place) if entropy else None
+        work, need = self._work(rows, actions)
         self._on_stream()
         _check(self._lib.omk_policy_logprobs(self._h, C.byref(r), d_moves, None if lp is None else lp.data_ptr(),
-                                             None if ent is None else ent.data_ptr(), None if work is None else work.data_ptr(), need))
+                                             None if ent is None else ent.data_ptr(),
+                                             None if work is None else work.data_ptr(), need))
         return Logprobs(lp, ent)
 
     def policy_loss(self, logits, moves, old_logprob, advantage, ref_logprob=None, weight=None, legal=None, clip_low=0.2,
@@ -263,10 +272,9 @@ class Learner:
         old_logprob, advantage, ref_logprob, weight: float32 [rows].  scale None: 1 / rows.  grad: True for a new tensor,
         False for none, or the tensor to write (the logits themselves are allowed).  Returns PolicyLoss(loss (one
         value), grad, logprob [rows], kl [rows])."""
-        torch = _torch()
         r, rows, actions = self._rows(logits, legal)
-        f32 = torch.float32
-        samples = _Samples(self._vector("moves", moves, rows, torch.int32), self._vector("old_logprob", old_logprob, rows, f32),
+        f32 = self._f32
+        samples = _Samples(self._vector("moves", moves, rows, self._i32), self._vector("old_logprob", old_logprob, rows, f32),
                            self._vector("advantage", advantage, rows, f32),
                            self._vector("ref_logprob", ref_logprob, rows, f32), self._vector("weight", weight, rows, f32))
         params = _PolicyParams(clip_low, clip_high, kl_weight, 1.0 / max(rows, 1) if scale is None else scale)
@@ -274,14 +282,15 @@ class Learner:
         need = self._lib.omk_policy_loss_work(rows, actions)
         # one allocation for what is small: log-probabilities, kl, the loss, and the work space behind them
         behind = (2 * rows + 4) // 4 * 4
-        small = torch.empty(behind + (need + 3) // 4, dtype=f32, device=logits.device)
+        small = self._empty(behind + (need + 3) // 4, dtype=f32, device=self._place)
         at = small.data_ptr()
         out = _PolicyOut(at + 8 * rows, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                          at + 4 * rows)
         self._on_stream()
         _check(self._lib.omk_policy_loss(self._h, C.byref(r), C.byref(samples), C.byref(params), C.byref(out),
                                          at + 4 * behind, need))
-        return PolicyLoss(small[2 * rows], g, small[:rows], small[rows:2 * rows])
+        view = small.as_strided
+        return PolicyLoss(view((), (), 2 * rows), g, view((rows,), (1,), 0), view((rows,), (1,), rows))
 
     def preference_loss(self, logits, moves, line_begin, ref_logprob=None, legal=None, beta=0.1, label_smoothing=0.0,
                         scale=None, grad=True):
@@ -291,28 +300,28 @@ class Learner:
         ref_logprob: float32 [2 * pairs], the lines' log-probabilities under the reference policy (grad=False on its
         logits gives them).  scale None: 1 / pairs.  grad: as in policy_loss; rows of no line are left as they are (a
         new tensor has zeros there).  Returns PreferenceLoss(loss, grad, margin [pairs], logprob [2 * pairs])."""
-        torch = _torch()
         r, rows, actions = self._rows(logits, legal)
-        f32 = torch.float32
+        f32 = self._f32
         if line_begin.dim() != 1 or line_begin.shape[0] % 2 != 1:
             raise ValueError("line_begin of shape %s: two lines a pair and the end" % (tuple(line_begin.shape),))
         lines = line_begin.shape[0] - 1
         pairs = lines // 2
-        d_begin = self._vector("line_begin", line_begin, lines + 1, torch.int32)
-        d_moves = self._vector("moves", moves, rows, torch.int32)
+        d_begin = self._vector("line_begin", line_begin, lines + 1, self._i32)
+        d_moves = self._vector("moves", moves, rows, self._i32)
         d_ref = self._vector("ref_logprob", ref_logprob, lines, f32)
         params = _PreferenceParams(beta, label_smoothing, 1.0 / max(pairs, 1) if scale is None else scale)
         g = self._gradient(grad, logits)
         need = self._lib.omk_preference_loss_work(rows, actions, pairs)
         behind = (3 * pairs + 4) // 4 * 4
-        small = torch.empty(behind + (need + 3) // 4, dtype=f32, device=logits.device)
+        small = self._empty(behind + (need + 3) // 4, dtype=f32, device=self._place)
         at = small.data_ptr()
         out = _PreferenceOut(at + 12 * pairs, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                              at + 4 * pairs, grad is True)
         self._on_stream()
         _check(self._lib.omk_preference_loss(self._h, C.byref(r), d_moves, d_begin, pairs, d_ref, C.byref(params),
                                              C.byref(out), at + 4 * behind, need))
-        return PreferenceLoss(small[3 * pairs], g, small[:pairs], small[pairs:3 * pairs])
+        view = small.as_strided
+        return PreferenceLoss(view((), (), 3 * pairs), g, view((pairs,), (1,), 0), view((lines,), (1,), pairs))
 
 
 class AdamW:
@@ -380,7 +389,7 @@ class AdamW:
                          _NONE if copy_type is None else kinds[copy_type], _F32 if states == "f32" else _F8,
                          float(betas[0]), float(betas[1]), float(eps), int(seed) & 0xFFFFFFFF)
         self._sizes = [p.numel() for p in self.params]
-        self._grads = (C.c_void_p * n)()
+        self._grads = C.c_void_p * n
         learner._on_stream()
         _check(self._lib.omk_adamw_create(learner._h, C.byref(desc), C.byref(self._h)))
 
@@ -401,23 +410,24 @@ class AdamW:
         value that gradients are multiplied by (a clipping factor, one over a loss scale)."""
         if len(grads) != len(self.params):
             raise ValueError("%d gradients of %d parameters" % (len(grads), len(self.params)))
-        learner, dtype, at = self.learner, self.grad_type, self._grads
-        for i, (g, n) in enumerate(zip(grads, self._sizes)):
+        learner, dtype, device = self.learner, self.grad_type, self.learner.device
+        at = []
+        for g, n in zip(grads, self._sizes):
             if g is None:
-                at[i] = None
-                continue
-            if g.dtype != dtype or g.numel() != n or not g.is_contiguous() or g.get_device() != learner.device:
+                at.append(None)
+            elif g.dtype is dtype and g.numel() == n and g.get_device() == device and g.is_contiguous():
+                at.append(g.data_ptr())
+            else:
                 raise ValueError("gradient %d: %s %s on %s: %d contiguous values of %s on device %d are wanted" %
-                                 (i, g.dtype, tuple(g.shape), g.device, n, dtype, learner.device))
-            at[i] = g.data_ptr()
+                                 (len(at), g.dtype, tuple(g.shape), g.device, n, dtype, device))
         d_lr, number = None, 0.0
         if isinstance(lr, (int, float)):
             number = lr
         else:
-            d_lr = learner._vector("lr", lr.reshape(-1), 1, _torch().float32)
-        d_scale = None if grad_scale is None else learner._vector("grad_scale", grad_scale.reshape(-1), 1, _torch().float32)
+            d_lr = learner._vector("lr", lr.reshape(-1), 1, learner._f32)
+        d_scale = None if grad_scale is None else learner._vector("grad_scale", grad_scale.reshape(-1), 1, learner._f32)
         learner._on_stream()
-        _check(self._lib.omk_adamw_step(self._h, at, number, d_lr, d_scale))
+        _check(self._lib.omk_adamw_step(self._h, self._grads(*at), number, d_lr, d_scale))
 
     def state(self):
         """The moments, as they are held: dict(m, v) and with 8-bit states (float8_e4m3fn, v's square root) m_scale and
