@@ -57,13 +57,29 @@ __device__ __forceinline__ uint32_t legal_bits(const uint32_t *legal, int words,
     return j < 0 ? bits << -j : bits;
 }
 
-template <typename T>
+// ONCE: the matrix is larger than the caches, and what is read or written now is not met again in them (nontemporal loads
+// and stores).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool ONCE>
+__device__ __forceinline__ uint4 load16(const void *from) {
+    if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u32x4 *)from));
+    return *(const uint4 *)from;
+}
+template <bool ONCE>
+__device__ __forceinline__ void store16(void *to, uint4 v) {
+    if constexpr (ONCE)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4 *)to);
+    else
+        *(uint4 *)to = v;
+}
+
+template <bool ONCE, typename T>
 __device__ __forceinline__ void load_vector(const Rows &r, int64_t row, int j, uint32_t inside, Pack<T> &p) {
     constexpr int V = Pack<T>::V;
     const int64_t at = row * r.stride + j;
     if (!inside) return;
     if (r.aligned && at + V <= r.span) {  // (at >= 0: the matrix begins at a multiple of 16 bytes)
-        p.raw = *(const uint4 *)((const T *)r.x + at);
+        p.raw = load16<ONCE>((const T *)r.x + at);
         return;
     }
 #pragma unroll
@@ -71,7 +87,7 @@ __device__ __forceinline__ void load_vector(const Rows &r, int64_t row, int j, u
         if (inside >> i & 1u) p.x[i] = ((const T *)r.x)[at + i];
 }
 
-template <typename T, typename OUT>
+template <bool ONCE, typename T, typename OUT>
 __device__ __forceinline__ void store_vector(OUT *out, bool aligned, int j, int actions, const float (&y)[Pack<T>::V]) {
     constexpr int V = Pack<T>::V;
     if (aligned && j >= 0 && j + V <= actions) {
@@ -79,10 +95,11 @@ __device__ __forceinline__ void store_vector(OUT *out, bool aligned, int j, int 
             Pack<OUT> p;
 #pragma unroll
             for (int i = 0; i < V; i++) p.x[i] = (OUT)y[i];
-            *(uint4 *)(out + j) = p.raw;
+            store16<ONCE>(out + j, p.raw);
         } else {  // 32-bit results of 16-bit logits
 #pragma unroll
-            for (int i = 0; i < V; i += 4) *(float4 *)(out + j + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+            for (int i = 0; i < V; i += 4)
+                store16<ONCE>(out + j + i, __builtin_bit_cast(uint4, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3])));
         }
         return;
     }
@@ -275,119 +292,271 @@ __device__ __forceinline__ RowStats join_waves(float top, double sum, float cent
     return all;
 }
 
-// TEAM lanes hold a row, K vectors each.  Up to 64 lanes: blocks of 256 threads, whose teams take rows of their
-// own; more: a block a row.
-template <typename T, int TEAM, int K, typename OP>
-__global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void k_rows(Rows r, OP op) {
+// exp(x - m) of a vector's elements and their sum; with CENTRED also adds exp(x - m) (x - m) up, where a term whose exponential
+// is 0 (x = -inf among them) counts nothing and one that is no number shows.
+template <bool CENTRED, int V>
+__device__ __forceinline__ float exponentials(const float (&x)[V], float top, float (&e)[V], float &centred) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float d = x[i] - top;
+        e[i] = exp_of(d);
+        if (CENTRED) centred = __builtin_fmaf(e[i], fmaxf(d, -200.0f), centred);
+    }
+    return sum_of<V>(e);
+}
+
+// The elements of a vector as floats, -inf where they are not the row's or not legal.  LOOK: nearly all vectors of a row
+// without a mask are whole in every lane, and need no look at single elements.  (Not where registers are short: two
+// ways through the code keep more alive.)
+template <bool LOOK, typename T>
+__device__ __forceinline__ void floats_of(const Pack<T> &p, uint32_t bits, float (&x)[Pack<T>::V]) {
     constexpr int V = Pack<T>::V;
-    constexpr int BLOCK = TEAM <= 64 ? 256 : TEAM, WAVES = BLOCK / 64, LANES = TEAM < 64 ? TEAM : 64;
-    constexpr bool KEEP = K * V <= 32;  // exp(x - m) stays in registers; wider rows compute it again from the logits
+    if (LOOK && __all(bits == (1u << V) - 1u)) {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = (float)p.x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = bits >> i & 1u ? (float)p.x[i] : -INFINITY;
+    }
+}
+
+// Writes a vector of a row's results: exp(x - m) times `each`, and `at_move` more at element `at` (counted from the first
+// vector's first; -1: nowhere), or 0.
+template <bool ONCE, typename T, typename OUT>
+__device__ __forceinline__ void write_vector(OUT *to, bool aligned, int vec, int head, int actions, const float (&e)[Pack<T>::V],
+                                             float each, bool none, int at, float at_move) {
+    constexpr int V = Pack<T>::V;
+    float y[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = none ? 0.0f : e[i] * each;
+    if (at >= 0 && at / V == vec) {
+#pragma unroll
+        for (int i = 0; i < V; i++) y[i] += at % V == i ? at_move : 0.0f;
+    }
+    store_vector<ONCE, T, OUT>(to, aligned, vec * V - head, actions, y);
+}
+
+// Narrow rows: TEAM lanes (of a wavefront's 64) hold R rows, K vectors of each a lane.  The few numbers of a row (its
+// log-probability, the loss and its slope: some 300 instructions, as many as a lane's share of the elements takes) are worked
+// out by one lane a row, for all the R rows at once.
+template <bool ONCE, typename T, int TEAM, int K, int R, typename OP>
+__global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
+    constexpr int V = Pack<T>::V;
     const int sub = threadIdx.x & (TEAM - 1);
-    const int64_t row = TEAM <= 64 ? (int64_t)blockIdx.x * (BLOCK / TEAM) + threadIdx.x / TEAM : (int64_t)blockIdx.x;
-    const bool here = row < r.rows;
-    const int head = here ? head_of<T>(r, row) : 0;
+    const int64_t base = ((int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM) * R;
+    // (loaded before this wavefront, which alone writes these rows' gradients, writes any: they may lie where the logits are)
+    const bool mine = sub < R && base + sub < r.rows;
+    Move m = {-1, -INFINITY};
+    if (OP::kMoves && mine) m = move_of<T>(r, op.moves, base + sub);
+    Pack<T> p[R][K];
+    uint32_t bits[R][K];
+#pragma unroll
+    for (int q = 0; q < R; q++) {
+        const bool here = base + q < r.rows;
+        const int head = here ? head_of<T>(r, base + q) : 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int j = (k * TEAM + sub) * V - head;
+            bits[q][k] = here ? inside_bits<V>(j, r.actions) : 0u;
+            load_vector<ONCE, T>(r, base + q, j, bits[q][k], p[q][k]);
+        }
+    }
+    if (r.legal) {
+#pragma unroll
+        for (int q = 0; q < R; q++) {
+            const int head = base + q < r.rows ? head_of<T>(r, base + q) : 0;
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                if (bits[q][k])
+                    bits[q][k] &= legal_bits(r.legal + (base + q) * r.legal_stride, r.words, (k * TEAM + sub) * V - head);
+        }
+    }
+    float e[R][K][V];
+    RowStats s = {0.0f, 0.0f, 0.0};
+#pragma unroll
+    for (int q = 0; q < R; q++) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            floats_of<true, T>(p[q][k], bits[q][k], e[q][k]);
+#pragma unroll
+            for (int i = 0; i < V; i++) top = fmaxf(top, e[q][k][i]);
+        }
+        top = team_max<TEAM>(top);
+        if (top == -INFINITY) top = 0.0f;
+        float sum = 0.0f, centred = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; k++) sum += exponentials<OP::kCentred, V>(e[q][k], top, e[q][k], centred);
+        const double all = team_sum<TEAM>((double)sum);
+        if (OP::kCentred) centred = team_sum<TEAM>(centred);
+        if (R == 1 || sub == q) s = {top, centred, all};
+    }
+    RowOut out = {0.0f, 0.0f, -1, true, 0.0f};
+    if (mine) out = op.row(base + sub, s, m, true);
+
+    if constexpr (OP::kElements) {
+        typedef typename OP::template Element<T> OUT;
+        if (op.template elements<OUT>(0)) {
+#pragma unroll
+            for (int q = 0; q < R; q++) {
+                const int head = base + q < r.rows ? head_of<T>(r, base + q) : 0;
+                const float each = __shfl(out.each, q, TEAM), at_move = __shfl(out.at_move, q, TEAM);
+                const int move = __shfl(out.move, q, TEAM);
+                const bool none = __shfl((int)out.none, q, TEAM);
+                OUT *to = op.template elements<OUT>(base + q);
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const int vec = k * TEAM + sub;
+                    if (base + q < r.rows && vec * V - head < r.actions)
+                        write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, e[q][k], each, none,
+                                                   move < 0 ? -1 : move + head, at_move);
+                }
+            }
+        }
+    }
+    if constexpr (OP::kLoss) {
+        __shared__ double shares[4];
+        const double share = team_sum<64>(mine ? (double)out.share : 0.0);
+        if ((threadIdx.x & 63) == 0) shares[threadIdx.x >> 6] = share;
+        __syncthreads();
+        if (threadIdx.x == 0) op.block_loss[blockIdx.x] = (float)(shares[0] + shares[1] + (shares[2] + shares[3]));
+    }
+}
+
+// Wider rows: a block of TEAM threads holds a row, K vectors a thread.
+//
+// What bounds it is memory's rate, if enough loads are on their way: a block that waits for its row's reductions loads
+// nothing, so a compute unit needs two of the largest blocks (at most 64 registers a thread).  8192 rows of 32768 bf16
+// with their gradient take 229 us with two (4.7 TB/s; 205 us with nontemporal accesses), 313 us with one.
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
+__global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(Rows r, OP op) {
+    constexpr int V = Pack<T>::V, WAVES = TEAM / 64;
+    // exp(x - m) stays in registers, up to 32 of them; wider rows compute it again from the logits
+    constexpr bool KEEP = K * V <= 32;
+    const int64_t row = blockIdx.x;
+    const int head = head_of<T>(r, row);
 
     // (the wavefront that looks at the move writes no other's part of the row before it has used what it found: the
     // gradient may lie where the logits are)
     Move m = {-1, -INFINITY};
-    if (OP::kMoves && here && (TEAM <= 64 || threadIdx.x < 64)) m = move_of<T>(r, op.moves, row);
+    if (OP::kMoves && threadIdx.x < 64) m = move_of<T>(r, op.moves, row);
     Pack<T> p[K];
     uint32_t bits[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const int j = (k * TEAM + sub) * V - head;
-        bits[k] = here ? inside_bits<V>(j, r.actions) : 0u;
-        load_vector<T>(r, row, j, bits[k], p[k]);
+        const int j = (k * TEAM + (int)threadIdx.x) * V - head;
+        bits[k] = inside_bits<V>(j, r.actions);
+        load_vector<ONCE, T>(r, row, j, bits[k], p[k]);
     }
-    if (r.legal && here) {
+    if (r.legal) {
         const uint32_t *legal = r.legal + row * r.legal_stride;
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (bits[k]) bits[k] &= legal_bits(legal, r.words, (k * TEAM + sub) * V - head);
+            if (bits[k]) bits[k] &= legal_bits(legal, r.words, (k * TEAM + (int)threadIdx.x) * V - head);
     }
-    const auto logit = [&](int k, int i) { return bits[k] >> i & 1u ? (float)p[k].x[i] : -INFINITY; };
-
+    float e[KEEP ? K : 1][V];
     float top = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < K; k++)
+    for (int k = 0; k < K; k++) {
+        float(&x)[V] = e[KEEP ? k : 0];
+        floats_of<false, T>(p[k], bits[k], x);
 #pragma unroll
-        for (int i = 0; i < V; i++) top = fmaxf(top, logit(k, i));
-    top = team_max<LANES>(top);
+        for (int i = 0; i < V; i++) top = fmaxf(top, x[i]);
+    }
+    top = team_max<64>(top);
     const float own_top = top == -INFINITY ? 0.0f : top;
-    float e[KEEP ? K : 1][V];
     float sum = 0.0f, centred = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        float t[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float d = logit(k, i) - own_top;
-            t[i] = exp_of(d);
-            if (OP::kCentred) centred += t[i] > 0.0f ? t[i] * d : 0.0f;
-            if (KEEP) e[k][i] = t[i];
-        }
-        sum += sum_of<V>(t);
+        float(&x)[V] = e[KEEP ? k : 0];
+        if (!KEEP) floats_of<false, T>(p[k], bits[k], x);
+        sum += exponentials<OP::kCentred, V>(x, own_top, x, centred);
     }
-    RowStats s = {own_top, 0.0f, team_sum<LANES>((double)sum)};
-    if (OP::kCentred) s.centred = team_sum<LANES>(centred);
-
-    float factor = 1.0f;  // from this wavefront's maximum to the row's
-    RowOut out;
-    if constexpr (TEAM <= 64) {
-        out = op.row(here ? row : 0, s, m, here && sub == 0);
-    } else {
-        __shared__ RowOut shared_out;
-        s = join_waves<OP::kCentred, WAVES>(top, s.sum, s.centred);
-        factor = top == -INFINITY ? 0.0f : exp_of(top - s.top);
-        if (threadIdx.x < 64) {
-            out = op.row(row, s, m, threadIdx.x == 0);
-            if (threadIdx.x == 0) shared_out = out;
-        }
-        if (OP::kElements) {
-            __syncthreads();
-            out = shared_out;
-        }
+    if (OP::kCentred) centred = team_sum<64>(centred);
+    __shared__ RowOut shared_out;
+    const RowStats s = join_waves<OP::kCentred, WAVES>(top, team_sum<64>((double)sum), centred);
+    if (threadIdx.x < 64) {
+        const RowOut o = op.row(row, s, m, threadIdx.x == 0);
+        if (threadIdx.x == 0) shared_out = o;
     }
-
     if constexpr (OP::kElements) {
+        __syncthreads();
         typedef typename OP::template Element<T> OUT;
-        OUT *to = op.template elements<OUT>(row);
-        if (to && here) {
-            const float each = out.each * factor;
-            const int at = out.move < 0 ? -1 : out.move + head;
+        const RowOut out = shared_out;
+        if (OUT *to = op.template elements<OUT>(row)) {
+            const float each = out.each * (top == -INFINITY ? 0.0f : exp_of(top - s.top));
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                const int vec = k * TEAM + sub, j = vec * V - head;
-                if (j >= r.actions) continue;
-                float y[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const float t = KEEP ? e[k][i] : exp_of(logit(k, i) - own_top);
-                    y[i] = out.none ? 0.0f : t * each;
+                const int vec = k * TEAM + (int)threadIdx.x;
+                float(&x)[V] = e[KEEP ? k : 0];
+                if (!KEEP) {
+                    floats_of<false, T>(p[k], bits[k], x);
+                    exponentials<false, V>(x, own_top, x, centred);
                 }
-                if (at >= 0 && at / V == vec) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) y[i] += at % V == i ? out.at_move : 0.0f;
-                }
-                store_vector<T, OUT>(to, op.aligned, j, r.actions, y);
+                if (vec * V - head < r.actions)
+                    write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, x, each, out.none,
+                                               out.move < 0 ? -1 : out.move + head, out.at_move);
             }
         }
     }
+    if (OP::kLoss && threadIdx.x == 0) op.block_loss[row] = shared_out.share;
+}
 
-    if constexpr (OP::kLoss) {
-        if constexpr (TEAM <= 64) {
-            __shared__ float shares[BLOCK / TEAM];
-            if (sub == 0) shares[threadIdx.x / TEAM] = here ? out.share : 0.0f;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                double all = 0.0;
-                for (int i = 0; i < BLOCK / TEAM; i++) all += (double)shares[i];
-                op.block_loss[blockIdx.x] = (float)all;
-            }
-        } else if (threadIdx.x == 0) {
-            op.block_loss[blockIdx.x] = out.share;
+// ---- rows of which nothing but numbers is wanted ----
+
+constexpr int kTile = 2;  // vectors of a thread at a time
+
+// A block goes through vectors first .. end - 1 of a row tile by tile with a running maximum and sum: m' = max(m, tile's
+// maximum), s' = s exp(m - m') + sum exp(x - m').  The next tile is on its way while one is looked at, and few registers hold
+// it all, so that eight blocks share a compute unit.  (Tiles of four vectors were slower by a tenth: five blocks.)
+template <bool ONCE, typename T, int BLOCK, bool CENTRED>
+__device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int first, int end) {
+    constexpr int V = Pack<T>::V;
+    const int head = head_of<T>(r, row);
+    const uint32_t *legal = r.legal ? r.legal + row * r.legal_stride : nullptr;
+    Pack<T> next[kTile];
+    const auto bits_at = [&](int vec) { return vec < end ? inside_bits<V>(vec * V - head, r.actions) : 0u; };
+    const auto load = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < kTile; k++)
+            load_vector<ONCE, T>(r, row, (from + k * BLOCK) * V - head, bits_at(from + k * BLOCK), next[k]);
+    };
+    load(first + (int)threadIdx.x);
+    float top = -INFINITY, sum = 0.0f, centred = 0.0f;
+    for (int start = first; start < end; start += kTile * BLOCK) {
+        const int from = start + (int)threadIdx.x;
+        float x[kTile][V], most = top;
+#pragma unroll
+        for (int k = 0; k < kTile; k++) {
+            uint32_t bits = bits_at(from + k * BLOCK);
+            if (legal && bits) bits &= legal_bits(legal, r.words, (from + k * BLOCK) * V - head);
+            floats_of<true, T>(next[k], bits, x[k]);
+#pragma unroll
+            for (int i = 0; i < V; i++) most = fmaxf(most, x[k][i]);
         }
+        load(from + kTile * BLOCK);
+        const float at = most == -INFINITY ? 0.0f : most, d = top - at, f = exp_of(d);
+        if (CENTRED) centred = top == -INFINITY ? 0.0f : (centred + sum * d) * f;
+        sum *= f;
+#pragma unroll
+        for (int k = 0; k < kTile; k++) sum += exponentials<CENTRED, V>(x[k], at, x[k], centred);
+        top = most;
     }
+    // the lanes' maxima and sums, then the wavefronts'
+    const float most = team_max<64>(top);
+    const float d = top == -INFINITY ? 0.0f : top - most, f = exp_of(d);
+    if (CENTRED) centred = team_sum<64>((centred + sum * d) * f);
+    return join_waves<CENTRED, BLOCK / 64>(most, team_sum<64>((double)(sum * f)), centred);
+}
+
+template <bool ONCE, typename T, int BLOCK, typename OP>
+__global__ __launch_bounds__(BLOCK) void k_stream(Rows r, OP op) {
+    const int64_t row = blockIdx.x;
+    const int vectors = (r.actions + head_of<T>(r, row) + Pack<T>::V - 1) / Pack<T>::V;
+    Move m = {-1, -INFINITY};
+    if (threadIdx.x < 64) m = move_of<T>(r, op.moves, row);
+    const RowStats s = stream_row<ONCE, T, BLOCK, OP::kCentred>(r, row, 0, vectors);
+    if (threadIdx.x < 64) op.row(row, s, m, threadIdx.x == 0);
 }
 
 // ---- rows cut into pieces ----
@@ -406,43 +575,11 @@ struct Wide {
     Move *moves;      // [rows]: looked up before any gradient is written where logits may be
 };
 
-template <typename T, typename OP>
+template <bool ONCE, typename T, typename OP>
 __global__ __launch_bounds__(kPieceBlock) void k_parts(Rows r, OP op, Wide w) {
-    constexpr int V = Pack<T>::V, K = kPieceVectors;
     const int64_t row = blockIdx.x / w.pieces;
-    const int piece = blockIdx.x % w.pieces, head = head_of<T>(r, row);
-    const int first = piece * (K * kPieceBlock) + threadIdx.x;
-    Pack<T> p[K];
-    uint32_t bits[K];
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int j = (first + k * kPieceBlock) * V - head;
-        bits[k] = inside_bits<V>(j, r.actions);
-        load_vector<T>(r, row, j, bits[k], p[k]);
-        if (r.legal && bits[k]) bits[k] &= legal_bits(r.legal + row * r.legal_stride, r.words, j);
-    }
-    const auto logit = [&](int k, int i) { return bits[k] >> i & 1u ? (float)p[k].x[i] : -INFINITY; };
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < K; k++)
-#pragma unroll
-        for (int i = 0; i < V; i++) top = fmaxf(top, logit(k, i));
-    top = team_max<64>(top);
-    const float own_top = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, centred = 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        float t[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float d = logit(k, i) - own_top;
-            t[i] = exp_of(d);
-            if (OP::kCentred) centred += t[i] > 0.0f ? t[i] * d : 0.0f;
-        }
-        sum += sum_of<V>(t);
-    }
-    if (OP::kCentred) centred = team_sum<64>(centred);
-    RowStats s = join_waves<OP::kCentred, kPieceBlock / 64>(top, team_sum<64>((double)sum), centred);
+    const int piece = blockIdx.x % w.pieces, first = piece * (kPieceVectors * kPieceBlock);
+    RowStats s = stream_row<ONCE, T, kPieceBlock, OP::kCentred>(r, row, first, first + kPieceVectors * kPieceBlock);
     if (threadIdx.x) return;
     if (s.sum == 0.0) s.top = -INFINITY;  // nothing here: no maximum for the row's
     w.parts[blockIdx.x] = s;
@@ -450,7 +587,7 @@ __global__ __launch_bounds__(kPieceBlock) void k_parts(Rows r, OP op, Wide w) {
 }
 
 // A block for every piece (for every row where an operator has no elements).
-template <typename T, typename OP>
+template <bool ONCE, typename T, typename OP>
 __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
     constexpr int V = Pack<T>::V, K = kPieceVectors;
     const int64_t row = OP::kElements ? blockIdx.x / w.pieces : blockIdx.x;
@@ -493,17 +630,12 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
             if (j >= r.actions) continue;
             Pack<T> p;
             uint32_t bits = inside_bits<V>(j, r.actions);
-            load_vector<T>(r, row, j, bits, p);
+            load_vector<ONCE, T>(r, row, j, bits, p);
             if (r.legal) bits &= legal_bits(r.legal + row * r.legal_stride, r.words, j);
-            float y[V];
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                y[i] = out.none || !(bits >> i & 1u) ? 0.0f : exp_of((float)p.x[i] - s.top) * out.each;
-            if (at >= 0 && at / V == vec) {
-#pragma unroll
-                for (int i = 0; i < V; i++) y[i] += at % V == i ? out.at_move : 0.0f;
-            }
-            store_vector<T, OUT>(to, op.aligned, j, r.actions, y);
+            float x[V], unused = 0.0f;
+            floats_of<true, T>(p, bits, x);
+            exponentials<false, V>(x, s.top, x, unused);
+            write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, x, out.each, out.none, at, out.at_move);
         }
     }
 }
@@ -517,11 +649,14 @@ template <int BLOCK>
 __device__ __forceinline__ double block_sum(const float *values, int64_t n) {
     __shared__ double part[BLOCK / 64];
     double s = 0.0;
-    // (four at a time, so that as many loads are on their way)
+    // (eight at a time, so that as many loads are on their way)
     int64_t i = threadIdx.x;
-    for (; i + 3 * BLOCK < n; i += 4 * BLOCK) {
-        const float a = values[i], b = values[i + BLOCK], c = values[i + 2 * BLOCK], d = values[i + 3 * BLOCK];
-        s += ((double)a + (double)b) + ((double)c + (double)d);
+    for (; i + 7 * BLOCK < n; i += 8 * BLOCK) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = values[i + k * BLOCK];
+#pragma unroll
+        for (int k = 0; k < 8; k++) s += (double)v[k];
     }
     for (; i < n; i += BLOCK) s += (double)values[i];
     s = team_sum<64>(s);
@@ -534,7 +669,7 @@ __device__ __forceinline__ double block_sum(const float *values, int64_t n) {
 
 // A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.  Rows are taken from the last to the first: those that the
 // look at all rows has read last are in the cache still.
-template <typename T>
+template <bool ONCE, typename T>
 __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces) {
     constexpr int V = Pack<T>::V, K = kGradientVectors;
     const int lane = threadIdx.x & 63;
@@ -559,7 +694,7 @@ __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p,
     for (int k = 0; k < K; k++) {
         const int j = (first + k * 64) * V - head;
         bits[k] = slope == 0.0f ? 0u : inside_bits<V>(j, r.actions);
-        load_vector<T>(r, row, j, bits[k], x[k]);
+        load_vector<ONCE, T>(r, row, j, bits[k], x[k]);
     }
     if (r.legal) {
 #pragma unroll
@@ -570,14 +705,10 @@ __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p,
     for (int k = 0; k < K; k++) {
         const int vec = first + k * 64, j = vec * V - head;
         if (j >= r.actions) continue;
-        float y[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) y[i] = bits[k] >> i & 1u ? exp_of((float)x[k].x[i] - top) * each : 0.0f;
-        if (at >= 0 && at / V == vec) {
-#pragma unroll
-            for (int i = 0; i < V; i++) y[i] += at % V == i ? slope : 0.0f;
-        }
-        store_vector<T, T>(to, aligned, j, r.actions, y);
+        float e[V], unused = 0.0f;
+        floats_of<true, T>(x[k], bits[k], e);
+        exponentials<false, V>(e, top, e, unused);
+        write_vector<ONCE, T, T>(to, aligned, vec, head, r.actions, e, each, slope == 0.0f, at, slope);
     }
 }
 
@@ -597,35 +728,73 @@ struct Launched {
     int64_t shares;
 };
 
-template <typename T, int TEAM, int K, typename OP>
-static Launched run_rows(const Rows &r, const OP &op, hipStream_t stream) {
-    constexpr int per_block = TEAM <= 64 ? 256 / TEAM : 1;
-    const int64_t blocks = (r.rows + per_block - 1) / per_block;
+template <bool ONCE, typename T, int TEAM, int K, int R, typename OP>
+static Launched launch_narrow(const Rows &r, const OP &op, hipStream_t stream) {
+    const int64_t per_block = 256 / TEAM * R, blocks = (r.rows + per_block - 1) / per_block;
     OP o = op;
     if constexpr (OP::kLoss)
         if (blocks == 1) o.block_loss = op.p.loss;  // its share is the loss
-    k_rows<T, TEAM, K, OP><<<(unsigned)blocks, TEAM <= 64 ? 256 : TEAM, 0, stream>>>(r, o);
+    k_narrow<ONCE, T, TEAM, K, R, OP><<<(unsigned)blocks, 256, 0, stream>>>(r, o);
     return {hipGetLastError(), blocks};
 }
 
+// Rows of a team at once: as many as 16 registers of a lane hold, where so many rows are left that the card is full of
+// teams all the same (eight wavefronts a compute unit); else one, which is done sooner.
+constexpr int64_t kFullOfTeams = 256 * 8;
+
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
+static Launched run_narrow(const Rows &r, const OP &op, hipStream_t stream) {
+    constexpr int R = 4 / K * (int)sizeof(T) / 4;
+    if constexpr (R > 1)
+        if (r.rows >= kFullOfTeams * (64 / TEAM) * R) return launch_narrow<ONCE, T, TEAM, K, R>(r, op, stream);
+    return launch_narrow<ONCE, T, TEAM, K, 1>(r, op, stream);
+}
+
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
+static Launched run_rows(const Rows &r, const OP &op, hipStream_t stream) {
+    OP o = op;
+    if constexpr (OP::kLoss)
+        if (r.rows == 1) o.block_loss = op.p.loss;
+    k_rows<ONCE, T, TEAM, K, OP><<<(unsigned)r.rows, TEAM, 0, stream>>>(r, o);
+    return {hipGetLastError(), r.rows};
+}
+
+template <bool ONCE, typename T, int BLOCK, typename OP>
+static Launched run_stream(const Rows &r, const OP &op, hipStream_t stream) {
+    k_stream<ONCE, T, BLOCK, OP><<<(unsigned)r.rows, BLOCK, 0, stream>>>(r, op);
+    return {hipGetLastError(), r.rows};
+}
+
 // The narrowest team that holds a row.
+template <bool ONCE, typename T, typename OP>
+static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_t stream) {
+    const int64_t n = vectors_of<T>(r);
+    if (n <= 32) return run_narrow<ONCE, T, 32, 1>(r, op, stream);
+    if (n <= 64) return run_narrow<ONCE, T, 64, 1>(r, op, stream);
+    if (n <= 128) return run_narrow<ONCE, T, 64, 2>(r, op, stream);
+    if (n <= 256) return run_narrow<ONCE, T, 64, 4>(r, op, stream);
+    if (n <= 512) return run_rows<ONCE, T, 256, 2>(r, op, stream);
+    if constexpr (OP::kElements) {
+        if (n <= 1024) return run_rows<ONCE, T, 256, 4>(r, op, stream);
+        if (n <= 2048) return run_rows<ONCE, T, 1024, 2>(r, op, stream);
+        if (n <= 4096) return run_rows<ONCE, T, 1024, 4>(r, op, stream);
+        if (n <= 8192) return run_rows<ONCE, T, 1024, 8>(r, op, stream);
+        if constexpr (sizeof(T) == 4)
+            if (n <= 16384) return run_rows<ONCE, T, 1024, 16>(r, op, stream);
+    } else if (n <= 16384) {
+        return r.rows <= 256 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
+    }
+    k_parts<ONCE, T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, op, w);
+    k_apply<ONCE, T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, op, w);
+    return {hipGetLastError(), r.rows};
+}
+
+// Logits that the second-level caches (4 MB on each of the card's eight dies) cannot hold together are not kept in them.
+static inline bool met_once(const Rows &r, int width) { return r.rows * (int64_t)r.actions * width > (int64_t)32 << 20; }
+
 template <typename T, typename OP>
 static Launched run(const Rows &r, const OP &op, const Wide &w, hipStream_t stream) {
-    const int64_t n = vectors_of<T>(r);
-    if (n <= 32) return run_rows<T, 32, 1>(r, op, stream);
-    if (n <= 64) return run_rows<T, 64, 1>(r, op, stream);
-    if (n <= 128) return run_rows<T, 64, 2>(r, op, stream);
-    if (n <= 256) return run_rows<T, 64, 4>(r, op, stream);
-    if (n <= 512) return run_rows<T, 256, 2>(r, op, stream);
-    if (n <= 1024) return run_rows<T, 256, 4>(r, op, stream);
-    if (n <= 2048) return run_rows<T, 1024, 2>(r, op, stream);
-    if (n <= 4096) return run_rows<T, 1024, 4>(r, op, stream);
-    if (n <= 8192) return run_rows<T, 1024, 8>(r, op, stream);
-    if constexpr (sizeof(T) == 4)
-        if (n <= 16384) return run_rows<T, 1024, 16>(r, op, stream);
-    k_parts<T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, op, w);
-    k_apply<T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, op, w);
-    return {hipGetLastError(), r.rows};
+    return met_once(r, sizeof(T)) ? run_class<true, T>(r, op, w, stream) : run_class<false, T>(r, op, w, stream);
 }
 
 // Work space of rows that are cut into pieces, at the end of what the caller gives (behind `before` bytes).
@@ -670,8 +839,12 @@ Launched type_lines(const Rows &r, const PreferenceLoss &p, int64_t before, hipS
 template <typename T>
 hipError_t type_line_gradient(const Rows &r, const PreferenceLoss &p, hipStream_t stream) {
     const int64_t pieces = (vectors_of<T>(r) + 64 * kGradientVectors - 1) / (64 * kGradientVectors);
-    k_line_gradient<T><<<(unsigned)((r.rows * pieces + 3) / 4), 256, 0, stream>>>(
-        r, p, aligned_with<T>(r, p.grad, p.grad_stride), (int)pieces);
+    const dim3 grid((unsigned)((r.rows * pieces + 3) / 4));
+    const bool aligned = aligned_with<T>(r, p.grad, p.grad_stride);
+    if (met_once(r, sizeof(T)))
+        k_line_gradient<true, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces);
+    else
+        k_line_gradient<false, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces);
     return hipGetLastError();
 }
 
