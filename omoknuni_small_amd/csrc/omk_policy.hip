@@ -14,20 +14,22 @@ __global__ __launch_bounds__(kSumBlock) void k_sum(const float *values, int64_t 
     if (threadIdx.x == 0) *out = (float)s;
 }
 
-// A wavefront for every pair of lines: the lines' sums, the pair's loss, and the slope of every row of theirs.
+// A block for every pair of lines, half of it a line: the lines' sums, the pair's loss, and the slope of every row of theirs.
 __global__ __launch_bounds__(256) void k_pairs(Rows r, PreferenceLoss p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (pair >= p.pairs) return;
-    double sums[2];
-    for (int side = 0; side < 2; side++) {
-        const int64_t line = 2 * pair + side;
-        const int64_t begin = inside_rows(p.line_begin[line], r.rows), end = inside_rows(p.line_begin[line + 1], r.rows);
-        double s = 0.0;
-        for (int64_t row = begin + lane; row < end; row += 64) s += p.logprob[row];
-        sums[side] = team_sum<64>(s);
-        if (lane == 0 && p.line_logprob) p.line_logprob[line] = (float)sums[side];
-        if (p.ref_logprob) sums[side] -= (double)p.ref_logprob[line];
+    const int64_t pair = blockIdx.x, line = 2 * pair + (threadIdx.x >> 7);
+    const int half = threadIdx.x & 127;
+    const int64_t begin = inside_rows(p.line_begin[line], r.rows), end = inside_rows(p.line_begin[line + 1], r.rows);
+    double s = 0.0;
+    for (int64_t row = begin + half; row < end; row += 128) s += p.logprob[row];
+    s = team_sum<64>(s);
+    __shared__ double parts[4];
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = s;
+    __syncthreads();
+    double sums[2] = {parts[0] + parts[1], parts[2] + parts[3]};
+    if (half == 0 && p.line_logprob) p.line_logprob[line] = (float)sums[threadIdx.x >> 7];
+    if (p.ref_logprob) {
+        sums[0] -= (double)p.ref_logprob[2 * pair];
+        sums[1] -= (double)p.ref_logprob[2 * pair + 1];
     }
     const float u = (float)((double)p.beta * (sums[0] - sums[1]));
     // log(1 + exp(-|u|)), of which both losses are made
@@ -37,17 +39,13 @@ __global__ __launch_bounds__(256) void k_pairs(Rows r, PreferenceLoss p) {
     const float lesser = t / (1.0f + t), greater = 1.0f / (1.0f + t);  // sigmoid(-|u|), sigmoid(|u|)
     const float above = u >= 0.0f ? greater : lesser, below = u >= 0.0f ? lesser : greater;  // sigmoid(u), sigmoid(-u)
     const float slope = -p.beta * p.scale * ((1.0f - p.smoothing) * below - p.smoothing * above);
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         if (p.margin) p.margin[pair] = u;
         p.pair_loss[pair] = p.scale * loss;
     }
     if (!p.grad) return;
-    for (int side = 0; side < 2; side++) {
-        const int64_t line = 2 * pair + side;
-        const int64_t begin = inside_rows(p.line_begin[line], r.rows), end = inside_rows(p.line_begin[line + 1], r.rows);
-        for (int64_t row = begin + lane; row < end; row += 64)
-            p.slope[row] = p.inverse[row] == 0.0f ? 0.0f : side ? -slope : slope;
-    }
+    for (int64_t row = begin + half; row < end; row += 128)
+        p.slope[row] = p.inverse[row] == 0.0f ? 0.0f : threadIdx.x >> 7 ? -slope : slope;
 }
 
 __global__ void k_set_float(float *to, float value) { *to = value; }
@@ -107,7 +105,7 @@ hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss 
         OMK_BY_TYPE(type, l = type_lines<T>(r, p, before, stream));
         if (l.error != hipSuccess) return l.error;
     }
-    k_pairs<<<(unsigned)((p.pairs + 3) / 4), 256, 0, stream>>>(r, p);
+    k_pairs<<<(unsigned)p.pairs, 256, 0, stream>>>(r, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (p.grad) {

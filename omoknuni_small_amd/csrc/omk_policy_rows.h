@@ -49,11 +49,19 @@ __device__ __forceinline__ uint32_t inside_bits(int j, int actions) {
     return b;
 }
 
-// Bits of the elements that are legal (of those that are the row's).
+// Bits of the elements that are legal (of those that are the row's): from two neighbouring words at once.
 __device__ __forceinline__ uint32_t legal_bits(const uint32_t *legal, int words, int j) {
-    const int at = j < 0 ? 0 : j, w = at >> 5;
-    const uint32_t lo = legal[min(w, words - 1)], hi = legal[min(w + 1, words - 1)];
-    const uint32_t bits = __builtin_amdgcn_alignbit(hi, lo, at & 31);
+    const int at = j < 0 ? 0 : j;
+    uint32_t bits;
+    if (words > 1) {
+        struct __attribute__((packed, aligned(4))) Pair {
+            uint64_t both;
+        };
+        const int w = min(at >> 5, words - 2);
+        bits = (uint32_t)(((const Pair *)(legal + w))->both >> (at - 32 * w));
+    } else {
+        bits = legal[0] >> at;
+    }
     return j < 0 ? bits << -j : bits;
 }
 
@@ -181,10 +189,10 @@ struct LogprobsOp {
     }
 };
 
-// exp(d) - d - 1 without the cancellation near 0: d^2/2 (1 + d/3 (1 + d/4 (..))), whose first term left out is below
-// 2^-24 of the sum for |d| < 1/4
-__device__ __forceinline__ float exp_minus_linear(float d, float expm1_d) {
-    if (fabsf(d) >= 0.25f) return expm1_d - d;
+// exp(d) - d - 1.  Near 0, where that cancels: d^2/2 (1 + d/3 (1 + d/4 (..))), whose first term left out is below 2^-24 of the
+// sum for |d| < 1/4.  (Added to d it is exp(d) - 1, which needs no call of its own.)
+__device__ __forceinline__ float exp_minus_linear(float d) {
+    if (fabsf(d) >= 0.25f) return (expf(d) - 1.0f) - d;
     float s = 1.0f + d * (1.0f / 9.0f);
     s = 1.0f + d * (1.0f / 8.0f) * s;
     s = 1.0f + d * (1.0f / 7.0f) * s;
@@ -220,10 +228,10 @@ struct PolicyOp {
                 loss = slope = -expf((float)shift) * a;
             }
             if (p.ref_logprob) {
-                const float d = (float)((double)p.ref_logprob[row] - exact), e = expm1f(d);
-                kl = exp_minus_linear(d, e);
+                const float d = (float)((double)p.ref_logprob[row] - exact);
+                kl = exp_minus_linear(d);
                 loss += p.kl_weight * kl;
-                slope -= p.kl_weight * e;
+                slope -= p.kl_weight * (d + kl);
             }
             const float w = (p.weight ? p.weight[row] : 1.0f) * p.scale;
             loss *= w;
@@ -316,7 +324,11 @@ __device__ __forceinline__ void floats_of(const Pack<T> &p, uint32_t bits, float
         for (int i = 0; i < V; i++) x[i] = (float)p.x[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) x[i] = bits >> i & 1u ? (float)p.x[i] : -INFINITY;
+        for (int i = 0; i < V; i++) {
+            // (the bit spread over a word, and the value or -inf picked by it: two instructions)
+            const uint32_t all = (uint32_t)((int32_t)(bits << (31 - i)) >> 31);
+            x[i] = __uint_as_float((__float_as_uint((float)p.x[i]) & all) | (0xFF800000u & ~all));
+        }
     }
 }
 
@@ -336,87 +348,68 @@ __device__ __forceinline__ void write_vector(OUT *to, bool aligned, int vec, int
     store_vector<ONCE, T, OUT>(to, aligned, vec * V - head, actions, y);
 }
 
-// Narrow rows: TEAM lanes (of a wavefront's 64) hold R rows, K vectors of each a lane.  The few numbers of a row (its
-// log-probability, the loss and its slope: some 300 instructions, as many as a lane's share of the elements takes) are worked
-// out by one lane a row, for all the R rows at once.
-template <bool ONCE, typename T, int TEAM, int K, int R, typename OP>
+// Narrow rows: TEAM lanes (of a wavefront's 64) hold a row, K vectors a lane.  What bounds it is the instructions, of which
+// elements are the smaller part: the reductions and a row's few numbers (its log-probability, the loss and its
+// slope: some 300) cost the same for a row in 8 lanes as for one in 64, and are shared by all rows of the wavefront.
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
 __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
     constexpr int V = Pack<T>::V;
     const int sub = threadIdx.x & (TEAM - 1);
-    const int64_t base = ((int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM) * R;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    const bool here = row < r.rows;
+    const int head = here ? head_of<T>(r, row) : 0;
     // (loaded before this wavefront, which alone writes these rows' gradients, writes any: they may lie where the logits are)
-    const bool mine = sub < R && base + sub < r.rows;
     Move m = {-1, -INFINITY};
-    if (OP::kMoves && mine) m = move_of<T>(r, op.moves, base + sub);
-    Pack<T> p[R][K];
-    uint32_t bits[R][K];
+    if (OP::kMoves && here && sub == 0) m = move_of<T>(r, op.moves, row);
+    Pack<T> p[K];
+    uint32_t bits[K];
 #pragma unroll
-    for (int q = 0; q < R; q++) {
-        const bool here = base + q < r.rows;
-        const int head = here ? head_of<T>(r, base + q) : 0;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int j = (k * TEAM + sub) * V - head;
-            bits[q][k] = here ? inside_bits<V>(j, r.actions) : 0u;
-            load_vector<ONCE, T>(r, base + q, j, bits[q][k], p[q][k]);
-        }
+    for (int k = 0; k < K; k++) {
+        const int j = (k * TEAM + sub) * V - head;
+        bits[k] = here ? inside_bits<V>(j, r.actions) : 0u;
+        load_vector<ONCE, T>(r, row, j, bits[k], p[k]);
     }
     if (r.legal) {
 #pragma unroll
-        for (int q = 0; q < R; q++) {
-            const int head = base + q < r.rows ? head_of<T>(r, base + q) : 0;
-#pragma unroll
-            for (int k = 0; k < K; k++)
-                if (bits[q][k])
-                    bits[q][k] &= legal_bits(r.legal + (base + q) * r.legal_stride, r.words, (k * TEAM + sub) * V - head);
-        }
+        for (int k = 0; k < K; k++)
+            if (bits[k]) bits[k] &= legal_bits(r.legal + row * r.legal_stride, r.words, (k * TEAM + sub) * V - head);
     }
-    float e[R][K][V];
-    RowStats s = {0.0f, 0.0f, 0.0};
+    float e[K][V], top = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < R; q++) {
-        float top = -INFINITY;
+    for (int k = 0; k < K; k++) {
+        floats_of<true, T>(p[k], bits[k], e[k]);
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            floats_of<true, T>(p[q][k], bits[q][k], e[q][k]);
-#pragma unroll
-            for (int i = 0; i < V; i++) top = fmaxf(top, e[q][k][i]);
-        }
-        top = team_max<TEAM>(top);
-        if (top == -INFINITY) top = 0.0f;
-        float sum = 0.0f, centred = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; k++) sum += exponentials<OP::kCentred, V>(e[q][k], top, e[q][k], centred);
-        const double all = team_sum<TEAM>((double)sum);
-        if (OP::kCentred) centred = team_sum<TEAM>(centred);
-        if (R == 1 || sub == q) s = {top, centred, all};
+        for (int i = 0; i < V; i++) top = fmaxf(top, e[k][i]);
     }
+    top = team_max<TEAM>(top);
+    if (top == -INFINITY) top = 0.0f;
+    float sum = 0.0f, centred = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++) sum += exponentials<OP::kCentred, V>(e[k], top, e[k], centred);
+    if (OP::kCentred) centred = team_sum<TEAM>(centred);
+    const RowStats s = {top, centred, team_sum<TEAM>((double)sum)};
     RowOut out = {0.0f, 0.0f, -1, true, 0.0f};
-    if (mine) out = op.row(base + sub, s, m, true);
+    if (here && sub == 0) out = op.row(row, s, m, true);
 
     if constexpr (OP::kElements) {
         typedef typename OP::template Element<T> OUT;
         if (op.template elements<OUT>(0)) {
+            const float each = __shfl(out.each, 0, TEAM), at_move = __shfl(out.at_move, 0, TEAM);
+            const int move = __shfl(out.move, 0, TEAM);
+            const bool none = __shfl((int)out.none, 0, TEAM);
+            OUT *to = op.template elements<OUT>(row);
 #pragma unroll
-            for (int q = 0; q < R; q++) {
-                const int head = base + q < r.rows ? head_of<T>(r, base + q) : 0;
-                const float each = __shfl(out.each, q, TEAM), at_move = __shfl(out.at_move, q, TEAM);
-                const int move = __shfl(out.move, q, TEAM);
-                const bool none = __shfl((int)out.none, q, TEAM);
-                OUT *to = op.template elements<OUT>(base + q);
-#pragma unroll
-                for (int k = 0; k < K; k++) {
-                    const int vec = k * TEAM + sub;
-                    if (base + q < r.rows && vec * V - head < r.actions)
-                        write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, e[q][k], each, none,
-                                                   move < 0 ? -1 : move + head, at_move);
-                }
+            for (int k = 0; k < K; k++) {
+                const int vec = k * TEAM + sub;
+                if (here && vec * V - head < r.actions)
+                    write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, e[k], each, none,
+                                               move < 0 ? -1 : move + head, at_move);
             }
         }
     }
     if constexpr (OP::kLoss) {
         __shared__ double shares[4];
-        const double share = team_sum<64>(mine ? (double)out.share : 0.0);
+        const double share = team_sum<64>((double)out.share);
         if ((threadIdx.x & 63) == 0) shares[threadIdx.x >> 6] = share;
         __syncthreads();
         if (threadIdx.x == 0) op.block_loss[blockIdx.x] = (float)(shares[0] + shares[1] + (shares[2] + shares[3]));
@@ -728,26 +721,14 @@ struct Launched {
     int64_t shares;
 };
 
-template <bool ONCE, typename T, int TEAM, int K, int R, typename OP>
-static Launched launch_narrow(const Rows &r, const OP &op, hipStream_t stream) {
-    const int64_t per_block = 256 / TEAM * R, blocks = (r.rows + per_block - 1) / per_block;
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
+static Launched run_narrow(const Rows &r, const OP &op, hipStream_t stream) {
+    const int64_t per_block = 256 / TEAM, blocks = (r.rows + per_block - 1) / per_block;
     OP o = op;
     if constexpr (OP::kLoss)
         if (blocks == 1) o.block_loss = op.p.loss;  // its share is the loss
-    k_narrow<ONCE, T, TEAM, K, R, OP><<<(unsigned)blocks, 256, 0, stream>>>(r, o);
+    k_narrow<ONCE, T, TEAM, K, OP><<<(unsigned)blocks, 256, 0, stream>>>(r, o);
     return {hipGetLastError(), blocks};
-}
-
-// Rows of a team at once: as many as 16 registers of a lane hold, where so many rows are left that the card is full of
-// teams all the same (eight wavefronts a compute unit); else one, which is done sooner.
-constexpr int64_t kFullOfTeams = 256 * 8;
-
-template <bool ONCE, typename T, int TEAM, int K, typename OP>
-static Launched run_narrow(const Rows &r, const OP &op, hipStream_t stream) {
-    constexpr int R = 4 / K * (int)sizeof(T) / 4;
-    if constexpr (R > 1)
-        if (r.rows >= kFullOfTeams * (64 / TEAM) * R) return launch_narrow<ONCE, T, TEAM, K, R>(r, op, stream);
-    return launch_narrow<ONCE, T, TEAM, K, 1>(r, op, stream);
 }
 
 template <bool ONCE, typename T, int TEAM, int K, typename OP>
@@ -765,14 +746,24 @@ static Launched run_stream(const Rows &r, const OP &op, hipStream_t stream) {
     return {hipGetLastError(), r.rows};
 }
 
-// The narrowest team that holds a row.
+// Wavefronts that fill the card: eight on each of 256 compute units.
+constexpr int64_t kFullOfRows = 256 * 8;
+
 template <bool ONCE, typename T, typename OP>
 static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_t stream) {
     const int64_t n = vectors_of<T>(r);
-    if (n <= 32) return run_narrow<ONCE, T, 32, 1>(r, op, stream);
-    if (n <= 64) return run_narrow<ONCE, T, 64, 1>(r, op, stream);
-    if (n <= 128) return run_narrow<ONCE, T, 64, 2>(r, op, stream);
-    if (n <= 256) return run_narrow<ONCE, T, 64, 4>(r, op, stream);
+    // Few rows are done soonest with a lane for every vector; where the card is full of wavefronts all the same, many
+    // rows to a wavefront.
+    if (n <= 256) {
+        const auto full = [&](int team) { return r.rows >= kFullOfRows * (64 / team); };
+        if (n <= 32 && full(16)) return run_narrow<ONCE, T, 16, 2>(r, op, stream);
+        if (n <= 32) return run_narrow<ONCE, T, 32, 1>(r, op, stream);
+        if (n <= 64 && full(16)) return run_narrow<ONCE, T, 16, 4>(r, op, stream);
+        if (n <= 64) return run_narrow<ONCE, T, 64, 1>(r, op, stream);
+        if (n <= 128 && full(32)) return run_narrow<ONCE, T, 32, 4>(r, op, stream);
+        if (n <= 128) return run_narrow<ONCE, T, 64, 2>(r, op, stream);
+        return run_narrow<ONCE, T, 64, 4>(r, op, stream);
+    }
     if (n <= 512) return run_rows<ONCE, T, 256, 2>(r, op, stream);
     if constexpr (OP::kElements) {
         if (n <= 1024) return run_rows<ONCE, T, 256, 4>(r, op, stream);

@@ -94,10 +94,13 @@ def policy_loss(rows, moves, old, advantage, ref, weight, clip_low, clip_high, k
         d_off = off + np.abs(d) * U
         # exp(d + t) - (d + t) - 1 is (exp(d) - d - 1) + (exp(d) - 1) t + exp(d) t^2 / 2 + .., |t| <= d_off: where d is 0 the
         # second term is all there is
-        kl_off = np.abs(np.expm1(d)) * d_off + np.exp(np.abs(d)) * d_off ** 2 + kl * 12 * U + (np.abs(np.expm1(d)) + np.abs(d)) * 4 * U * (np.abs(d) >= 0.25)
+        kl_off = np.abs(np.expm1(d)) * d_off + np.exp(np.abs(d)) * d_off ** 2 + kl * 12 * U + (np.exp(d) + np.abs(d) + 1) * 4 * U * (np.abs(d) >= 0.25)
         row, row_off = row + kl_weight * kl, row_off + kl_weight * (kl_off + 3 * U * kl)
         slope = slope - kl_weight * np.expm1(d)
-        slope_off = slope_off + kl_weight * (np.exp(d) * d_off + 6 * U * np.abs(np.expm1(d)))
+        # exp(d) - 1 as d and exp(d) - d - 1 added: the rounding of exp(d) (two steps) and of the differences, of magnitudes up to
+        # exp(d) + |d| + 1
+        slope_off = slope_off + kl_weight * (np.exp(d) * d_off + 6 * U * np.abs(np.expm1(d)) +
+                                             (np.abs(d) >= 0.25) * 6 * U * (np.exp(d) + np.abs(d) + 1))
     w = weight * scale
     slope_off = slope_off + 3 * U * np.abs(slope)
     # a ratio within rounding of a border may fall on either side of it: the loss has the same value there, but not the slope
