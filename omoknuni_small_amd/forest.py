@@ -462,6 +462,21 @@ class Batch:
         self.forest.node_count()
         return first
 
+    def expand_logits(self, move_begin, moves, logits, learner, widening=None):
+        """expand_ex() with the priors that the network's logits give: logits [n, action_space] are on the GPU (a row a
+        traversal, as learner.priors takes them), and a leaf's priors are their softmax over the moves it offers.
+        Waits for the logits."""
+        from .learn import legal_of_moves
+        n = len(move_begin) - 1
+        if logits.dim() != 2 or logits.shape[0] != n:
+            raise ValueError("logits of shape %s for %d traversals" % (tuple(logits.shape), n))
+        actions = int(logits.shape[1])
+        if n * actions > np.iinfo(np.int32).max:
+            raise ValueError("%d x %d logits: more than offsets of 32 bits reach" % (n, actions))
+        legal = learner.upload_legal(legal_of_moves(move_begin, moves, actions))
+        policy = learner.priors(logits, legal=legal).cpu().numpy()
+        return self.expand_ex(move_begin, moves, np.arange(n + 1, dtype=np.int32) * actions, policy, actions, widening)
+
     def truncated(self):
         c = C.c_int32()
         _check(self._lib.omk_batch_truncated(self._h, C.byref(c)))

@@ -232,6 +232,10 @@ class Learner:
         need = self._lib.omk_policy_work(rows, actions)
         return (self._empty(need, dtype=self._torch.uint8, device=self._place), need) if need else (None, 0)
 
+    def upload_legal(self, mask):
+        """Masks of uint32 words in host memory (legal_of_moves) as `legal` takes them."""
+        return self._torch.from_numpy(np.ascontiguousarray(mask).view(np.int32)).to(self._place)
+
     # ---- operators ----
 
     def priors(self, logits, legal=None, out=None):
