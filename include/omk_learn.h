@@ -42,6 +42,7 @@ typedef enum omk_type {
 } omk_type;
 
 #define OMK_MAX_ACTIONS (1 << 24)
+#define OMK_MAX_PAIRS (1 << 23)
 
 typedef struct omk_learner omk_learner;
 typedef struct omk_adamw omk_adamw;
@@ -57,7 +58,8 @@ int omk_learner_sync(omk_learner *l);
 
 typedef struct omk_policy_rows {
     const void *d_logits;    /* row r, action j at element r * row_stride + j */
-    int64_t row_stride;      /* elements; at least `actions` when there is more than one row */
+    int64_t row_stride;      /* elements; at least `actions` when there is more than one row.  What lies between
+                                two rows may be read, and is not looked at */
     int64_t rows;            /* 0 .. 2^31 - 1; with 0 every call returns OMK_OK (a loss is then set to 0) */
     int32_t actions;         /* 1 .. OMK_MAX_ACTIONS */
     int32_t type;            /* OMK_F32, OMK_BF16, OMK_F16 */
@@ -117,8 +119,10 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
  * count nothing) and u_k = beta * ((S_2k - ref_2k) - (S_2k+1 - ref_2k+1)):
  *   loss = scale * sum over pairs of -(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)
  * d_ref_logprob[s] = the line's sum under the reference policy (NULL: 0); a call without d_grad on the reference's logits
- * gives it as d_line_logprob.  d_line_begin must not decrease; bounds outside [0, rows] are taken as 0 or rows, and
- * a line that would end before it begins is empty.  Rows of no line are not read. */
+ * gives it as d_line_logprob.  d_line_begin must not decrease.  (Bounds that do not fit are taken as the nearest that
+ * do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
+ * empty; which line's gradient a row of two lines gets is open.)  Rows before the first line and behind the last are not
+ * read.  0 .. OMK_MAX_PAIRS pairs. */
 typedef struct omk_preference_params {
     double beta;
     double label_smoothing; /* 0 .. 0.5 */
@@ -166,7 +170,7 @@ typedef struct omk_adamw_desc {
     uint32_t seed;
 } omk_adamw_desc;
 /* Copies the description to the device; the tensors stay the caller's, and where they are.  Pointers need the alignment of
- * their type only.  Waits for the copy. */
+ * their type only; two that overlap are refused, a tensor that is there twice among them.  Waits for the copy. */
 int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out);
 /* Waits for the device.  (An optimizer whose learner has been destroyed only waits to be destroyed itself.) */
 int omk_adamw_destroy(omk_adamw *o);

@@ -141,7 +141,9 @@ __device__ __forceinline__ void store4(void *to, int64_t base, int lane, int the
     }
 }
 
-// A thread takes four elements, a wavefront a unit of 256, kUnitsAtOnce of them at a time.
+// A thread takes four elements, a wavefront a unit of 256, kUnitsAtOnce of them at a time: what bounds the step is memory's rate,
+// and with it the loads on their way.  95 M weights with bf16 gradients and copies: 492 us with 32-bit moments (28 bytes a
+// weight, 5.4 TB/s), 348 us with 8-bit ones (16 bytes, 4.4 TB/s); with two units at once 527 and 412 us, with eight 521 and 384 us.
 constexpr int kUnitsAtOnce = 4;
 
 // COUNT units of a tensor from `unit` on; all loads are on their way before the first is needed.  WHOLE: all their elements are

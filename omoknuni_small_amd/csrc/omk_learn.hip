@@ -6,6 +6,7 @@
 #include <cstring>
 #include <exception>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "omk_learn_internal.h"
@@ -66,10 +67,10 @@ int width_of(int type) { return type == OMK_F32 ? 4 : type == OMK_F8 ? 1 : 2; }
 bool float_type(int type) { return type == OMK_F32 || type == OMK_BF16 || type == OMK_F16; }
 bool aligned(const void *p, int width) { return ((uintptr_t)p & (uintptr_t)(width - 1)) == 0; }
 
-// Bytes from the first element of a matrix to behind its last; -1 where that passes 62 bits.
+// Bytes from the first element of a matrix to behind its last; -1 where that passes 2^46, which no address space holds.
 int64_t span_bytes(int64_t rows, int64_t stride, int64_t columns, int width) {
     const __int128 n = ((__int128)(rows - 1) * stride + columns) * width;
-    return n >> 62 ? -1 : (int64_t)n;
+    return n >> 46 ? -1 : (int64_t)n;
 }
 
 bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
@@ -94,7 +95,7 @@ int check_rows(const char *who, const omk_policy_rows *r, Rows *out) {
     if (r->rows && (span_bytes(r->rows, r->row_stride, r->actions, width_of(r->type)) < 0 ||
                     (r->d_legal && span_bytes(r->rows, r->legal_stride, words, 4) < 0)))
         return learn_fail(OMK_ERR_INVALID, "%s: rows that pass the address space", who);
-    *out = Rows{r->d_logits, r->row_stride, r->rows, r->actions, r->d_legal, r->legal_stride, words,
+    *out = Rows{r->d_logits, r->row_stride, r->rows, r->actions, 0, r->d_legal, r->legal_stride, words,
                 r->rows ? (r->rows - 1) * r->row_stride + r->actions : 0, aligned(r->d_logits, 16)};
     return OMK_OK;
 }
@@ -285,7 +286,7 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
     if (!l || !rows || !params || !out) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
     Rows r;
     if (int rc = check_rows(who, rows, &r)) return rc;
-    if (pairs < 0 || pairs > INT32_MAX / 2) return learn_fail(OMK_ERR_INVALID, "%s: %lld pairs", who, (long long)pairs);
+    if (pairs < 0 || pairs > OMK_MAX_PAIRS) return learn_fail(OMK_ERR_INVALID, "%s: %lld pairs", who, (long long)pairs);
     if (!std::isfinite(params->beta) || !std::isfinite(params->scale) || !(params->label_smoothing >= 0.0) ||
         !(params->label_smoothing <= 0.5))
         return learn_fail(OMK_ERR_INVALID, "%s: beta %g, label_smoothing %g (0 .. 0.5), scale %g", who, params->beta,
@@ -395,6 +396,20 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     first_chunk[(size_t)desc->n_tensors] = n_chunks;
     if (units > UINT32_MAX || n_chunks > INT32_MAX)
         return learn_fail(OMK_ERR_CAPACITY, "%s: over 2^40 elements", who);
+    // Every element is stepped once: what is stepped lies at one place each.
+    std::vector<std::pair<uintptr_t, uintptr_t>> places;
+    places.reserve((size_t)desc->n_tensors * 6);
+    for (const AdamTensor &t : tensors) {
+        const int64_t n = t.n, scales = (n + kUnit - 1) / kUnit * 4;
+        const std::pair<const void *, int64_t> all[] = {{t.param, n * width_of(pt)}, {t.copy, n * 2}, {t.m, n * width_of(st)},
+                                                        {t.v, n * width_of(st)}, {t.m_scale, scales}, {t.v_scale, scales}};
+        for (int i = 0; i < (st == OMK_F8 ? 6 : 4); i++)
+            if (n && all[i].first) places.emplace_back((uintptr_t)all[i].first, (uintptr_t)all[i].first + (uintptr_t)all[i].second);
+    }
+    std::sort(places.begin(), places.end());
+    for (size_t i = 1; i < places.size(); i++)
+        if (places[i].first < places[i - 1].second)
+            return learn_fail(OMK_ERR_INVALID, "%s: tensors that overlap at %p", who, (const void *)places[i].first);
     std::vector<AdamChunk> chunks((size_t)n_chunks);
     for (int32_t i = 0; i < desc->n_tensors; i++)
         for (int64_t c = first_chunk[i]; c < first_chunk[i + 1]; c++)

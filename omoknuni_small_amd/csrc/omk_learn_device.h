@@ -9,13 +9,18 @@ namespace omk {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-constexpr float kLog2E = 1.44269504088896341f;
+constexpr float kLog2E = 1.44269504088896341f, kLog2ELow = (float)(1.44269504088896341 - (double)1.44269504088896341f);
 constexpr double kLn2 = 0.693147180559945309417;
 
-// exp(x) of a difference to the row's largest logit: one product and v_exp_f32 (2^x, good to a unit in the last place).
-// The product's rounding makes exp(x) off by |x| 2^-24 relative: nothing where the value counts, since it is
-// exp(x) itself that gets small.  Below 2^-126 the result may be flushed to 0: 1e-38 of the largest term.
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
+// exp(x) of a difference to the row's largest logit, by 2^y of v_exp_f32 (good to a unit in the last place).  FINE: log2(e) in
+// two parts.  With the first alone all of a row's terms are off the same way, by 1.3e-8 |x|: nothing for a gradient, but
+// a line's log-probability adds hundreds of rows up (its margin was 2e-6 off, 3e-7 with both).  The second costs an
+// instruction in nine.  What is left is the rounding of the product, |x| 2^-24 relative: little where the value counts,
+// since it is exp(x) itself that gets small.  Below 2^-126 the result may be flushed to 0.
+template <bool FINE>
+__device__ __forceinline__ float exp_of(float x) {
+    return __builtin_amdgcn_exp2f(FINE ? __builtin_fmaf(x, kLog2E, x * kLog2ELow) : x * kLog2E);
+}
 
 // A reduction over teams of 8 .. 64 neighbouring lanes, the result in every lane of the team: lanes of a row of 16 by quad
 // swaps and mirrors, rows and halves by exchanging them.  (All 64 lanes are active where these are called.)

@@ -18,7 +18,8 @@ __global__ __launch_bounds__(kSumBlock) void k_sum(const float *values, int64_t 
 __global__ __launch_bounds__(256) void k_pairs(Rows r, PreferenceLoss p) {
     const int64_t pair = blockIdx.x, line = 2 * pair + (threadIdx.x >> 7);
     const int half = threadIdx.x & 127;
-    const int64_t begin = inside_rows(p.line_begin[line], r.rows), end = inside_rows(p.line_begin[line + 1], r.rows);
+    const LineRows lines = line_rows(p, r.rows);
+    const int64_t begin = lines.inside(p.line_begin[line]), end = lines.inside(p.line_begin[line + 1]);
     double s = 0.0;
     for (int64_t row = begin + half; row < end; row += 128) s += p.logprob[row];
     s = team_sum<64>(s);

@@ -166,6 +166,7 @@ struct PriorsOp {
     __device__ OUT *elements(int64_t row) const {
         return priors + row * stride;
     }
+    __device__ bool skips(const Rows &, int64_t) const { return false; }
     __device__ RowOut row(int64_t, const RowStats &s, Move, bool) const {
         return {s.sum == 0.0 ? 0.0f : 1.0f / (float)s.sum, 0.0f, -1, s.sum == 0.0, 0.0f};
     }
@@ -176,6 +177,7 @@ struct LogprobsOp {
     const int32_t *moves;
     float *block_loss;  // nullptr
     float *logprob, *entropy;
+    __device__ bool skips(const Rows &, int64_t) const { return false; }
     __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
         if (writes) {
             const double log_sum = log_of_sum(s.sum);
@@ -211,6 +213,7 @@ struct PolicyOp {
     float *block_loss;  // a block's share of the loss, by the block's number (by the row where rows are cut)
     PolicyLoss p;
     bool aligned;
+    __device__ bool skips(const Rows &, int64_t) const { return false; }
     template <typename OUT>
     __device__ OUT *elements(int64_t row) const {
         return p.grad ? (OUT *)p.grad + row * p.grad_stride : nullptr;
@@ -245,11 +248,26 @@ struct PolicyOp {
     }
 };
 
+// The rows that lines hold: from line_begin's first to its last, inside the rows there are.
+struct LineRows {
+    int64_t begin, end;
+    __device__ int64_t inside(int64_t at) const { return at < begin ? begin : at > end ? end : at; }
+};
+__device__ __forceinline__ LineRows line_rows(const PreferenceLoss &p, int64_t rows) {
+    const LineRows all = {0, rows};
+    const int64_t begin = all.inside(p.line_begin[0]), end = all.inside(p.line_begin[2 * p.pairs]);
+    return {begin, end < begin ? begin : end};
+}
+
 struct LineOp {
     static constexpr bool kCentred = false, kElements = false, kMoves = true, kLoss = false;
     const int32_t *moves;
     float *block_loss;  // nullptr
     PreferenceLoss p;
+    __device__ bool skips(const Rows &r, int64_t row) const {
+        const LineRows lines = line_rows(p, r.rows);
+        return row < lines.begin || row >= lines.end;
+    }
     __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
         if (writes) {
             const bool counts = m.chosen != -INFINITY;
@@ -261,15 +279,6 @@ struct LineOp {
         return {0.0f, 0.0f, -1, true, 0.0f};
     }
 };
-
-// The rows that lines hold: line_begin's first to its last, inside the rows there are.
-struct LineRows {
-    int64_t begin, end;
-};
-__device__ __forceinline__ int64_t inside_rows(int64_t at, int64_t rows) { return at < 0 ? 0 : at > rows ? rows : at; }
-__device__ __forceinline__ LineRows line_rows(const PreferenceLoss &p, int64_t rows) {
-    return {inside_rows(p.line_begin[0], rows), inside_rows(p.line_begin[2 * p.pairs], rows)};
-}
 
 // ---- rows that registers hold ----
 
@@ -293,7 +302,7 @@ __device__ __forceinline__ RowStats join_waves(float top, double sum, float cent
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
         const bool empty = tops[w] == -INFINITY;  // (its sum is 0, or NaN)
-        const float d = empty ? 0.0f : tops[w] - all.top, f = exp_of(d);
+        const float d = empty ? 0.0f : tops[w] - all.top, f = exp_of<true>(d);
         all.sum += sums[w] * (double)f;
         if (CENTRED) all.centred += (centreds[w] + (float)sums[w] * d) * f;
     }
@@ -302,12 +311,12 @@ __device__ __forceinline__ RowStats join_waves(float top, double sum, float cent
 
 // exp(x - m) of a vector's elements and their sum; with CENTRED also adds exp(x - m) (x - m) up, where a term whose exponential
 // is 0 (x = -inf among them) counts nothing and one that is no number shows.
-template <bool CENTRED, int V>
+template <bool FINE, bool CENTRED, int V>
 __device__ __forceinline__ float exponentials(const float (&x)[V], float top, float (&e)[V], float &centred) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const float d = x[i] - top;
-        e[i] = exp_of(d);
+        e[i] = exp_of<FINE>(d);
         if (CENTRED) centred = __builtin_fmaf(e[i], fmaxf(d, -200.0f), centred);
     }
     return sum_of<V>(e);
@@ -355,8 +364,8 @@ template <bool ONCE, typename T, int TEAM, int K, typename OP>
 __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
     constexpr int V = Pack<T>::V;
     const int sub = threadIdx.x & (TEAM - 1);
-    const int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
-    const bool here = row < r.rows;
+    const int64_t row = r.first + (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    const bool here = row < r.rows && !op.skips(r, row);
     const int head = here ? head_of<T>(r, row) : 0;
     // (loaded before this wavefront, which alone writes these rows' gradients, writes any: they may lie where the logits are)
     Move m = {-1, -INFINITY};
@@ -385,7 +394,7 @@ __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f, centred = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; k++) sum += exponentials<OP::kCentred, V>(e[k], top, e[k], centred);
+    for (int k = 0; k < K; k++) sum += exponentials<true, OP::kCentred, V>(e[k], top, e[k], centred);
     if (OP::kCentred) centred = team_sum<TEAM>(centred);
     const RowStats s = {top, centred, team_sum<TEAM>((double)sum)};
     RowOut out = {0.0f, 0.0f, -1, true, 0.0f};
@@ -420,13 +429,14 @@ __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
 //
 // What bounds it is memory's rate, if enough loads are on their way: a block that waits for its row's reductions loads
 // nothing, so a compute unit needs two of the largest blocks (at most 64 registers a thread).  8192 rows of 32768 bf16
-// with their gradient take 229 us with two (4.7 TB/s; 205 us with nontemporal accesses), 313 us with one.
+// with their gradient take 204 to 214 us with two (5.0 to 5.3 TB/s), 313 us with one (229 without nontemporal accesses).
 template <bool ONCE, typename T, int TEAM, int K, typename OP>
 __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(Rows r, OP op) {
     constexpr int V = Pack<T>::V, WAVES = TEAM / 64;
     // exp(x - m) stays in registers, up to 32 of them; wider rows compute it again from the logits
     constexpr bool KEEP = K * V <= 32;
-    const int64_t row = blockIdx.x;
+    const int64_t row = r.first + blockIdx.x;
+    if (op.skips(r, row)) return;
     const int head = head_of<T>(r, row);
 
     // (the wavefront that looks at the move writes no other's part of the row before it has used what it found: the
@@ -463,7 +473,7 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
     for (int k = 0; k < K; k++) {
         float(&x)[V] = e[KEEP ? k : 0];
         if (!KEEP) floats_of<false, T>(p[k], bits[k], x);
-        sum += exponentials<OP::kCentred, V>(x, own_top, x, centred);
+        sum += exponentials<!OP::kElements, OP::kCentred, V>(x, own_top, x, centred);
     }
     if (OP::kCentred) centred = team_sum<64>(centred);
     __shared__ RowOut shared_out;
@@ -477,14 +487,14 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
         typedef typename OP::template Element<T> OUT;
         const RowOut out = shared_out;
         if (OUT *to = op.template elements<OUT>(row)) {
-            const float each = out.each * (top == -INFINITY ? 0.0f : exp_of(top - s.top));
+            const float each = out.each * (top == -INFINITY ? 0.0f : exp_of<true>(top - s.top));
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int vec = k * TEAM + (int)threadIdx.x;
                 float(&x)[V] = e[KEEP ? k : 0];
                 if (!KEEP) {
                     floats_of<false, T>(p[k], bits[k], x);
-                    exponentials<false, V>(x, own_top, x, centred);
+                    exponentials<false, false, V>(x, own_top, x, centred);
                 }
                 if (vec * V - head < r.actions)
                     write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, x, each, out.none,
@@ -492,7 +502,7 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
             }
         }
     }
-    if (OP::kLoss && threadIdx.x == 0) op.block_loss[row] = shared_out.share;
+    if (OP::kLoss && threadIdx.x == 0) op.block_loss[blockIdx.x] = shared_out.share;
 }
 
 // ---- rows of which nothing but numbers is wanted ----
@@ -501,7 +511,8 @@ constexpr int kTile = 2;  // vectors of a thread at a time
 
 // A block goes through vectors first .. end - 1 of a row tile by tile with a running maximum and sum: m' = max(m, tile's
 // maximum), s' = s exp(m - m') + sum exp(x - m').  The next tile is on its way while one is looked at, and few registers hold
-// it all, so that eight blocks share a compute unit.  (Tiles of four vectors were slower by a tenth: five blocks.)
+// it all, so that eight blocks share a compute unit.  (Tiles of four vectors were slower by a tenth: five blocks.)  2049 rows of 50001
+// f16 with their entropies: 51 us, 4.0 TB/s.
 template <bool ONCE, typename T, int BLOCK, bool CENTRED>
 __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int first, int end) {
     constexpr int V = Pack<T>::V;
@@ -528,23 +539,24 @@ __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int f
             for (int i = 0; i < V; i++) most = fmaxf(most, x[k][i]);
         }
         load(from + kTile * BLOCK);
-        const float at = most == -INFINITY ? 0.0f : most, d = top - at, f = exp_of(d);
+        const float at = most == -INFINITY ? 0.0f : most, d = top - at, f = exp_of<true>(d);
         if (CENTRED) centred = top == -INFINITY ? 0.0f : (centred + sum * d) * f;
         sum *= f;
 #pragma unroll
-        for (int k = 0; k < kTile; k++) sum += exponentials<CENTRED, V>(x[k], at, x[k], centred);
+        for (int k = 0; k < kTile; k++) sum += exponentials<true, CENTRED, V>(x[k], at, x[k], centred);
         top = most;
     }
     // the lanes' maxima and sums, then the wavefronts'
     const float most = team_max<64>(top);
-    const float d = top == -INFINITY ? 0.0f : top - most, f = exp_of(d);
+    const float d = top == -INFINITY ? 0.0f : top - most, f = exp_of<true>(d);
     if (CENTRED) centred = team_sum<64>((centred + sum * d) * f);
     return join_waves<CENTRED, BLOCK / 64>(most, team_sum<64>((double)(sum * f)), centred);
 }
 
 template <bool ONCE, typename T, int BLOCK, typename OP>
 __global__ __launch_bounds__(BLOCK) void k_stream(Rows r, OP op) {
-    const int64_t row = blockIdx.x;
+    const int64_t row = r.first + blockIdx.x;
+    if (op.skips(r, row)) return;
     const int vectors = (r.actions + head_of<T>(r, row) + Pack<T>::V - 1) / Pack<T>::V;
     Move m = {-1, -INFINITY};
     if (threadIdx.x < 64) m = move_of<T>(r, op.moves, row);
@@ -571,6 +583,7 @@ struct Wide {
 template <bool ONCE, typename T, typename OP>
 __global__ __launch_bounds__(kPieceBlock) void k_parts(Rows r, OP op, Wide w) {
     const int64_t row = blockIdx.x / w.pieces;
+    if (op.skips(r, row)) return;
     const int piece = blockIdx.x % w.pieces, first = piece * (kPieceVectors * kPieceBlock);
     RowStats s = stream_row<ONCE, T, kPieceBlock, OP::kCentred>(r, row, first, first + kPieceVectors * kPieceBlock);
     if (threadIdx.x) return;
@@ -584,6 +597,7 @@ template <bool ONCE, typename T, typename OP>
 __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
     constexpr int V = Pack<T>::V, K = kPieceVectors;
     const int64_t row = OP::kElements ? blockIdx.x / w.pieces : blockIdx.x;
+    if (op.skips(r, row)) return;
     const int piece = OP::kElements ? blockIdx.x % w.pieces : 0;
     const RowStats *parts = w.parts + row * w.pieces;
     // a thread's parts, then its wavefront's, then the block's
@@ -594,7 +608,7 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
     float centred = 0.0f;
     for (int i = threadIdx.x; i < w.pieces; i += kPieceBlock) {
         const bool empty = parts[i].top == -INFINITY;
-        const float d = empty ? 0.0f : parts[i].top - top, f = exp_of(d);
+        const float d = empty ? 0.0f : parts[i].top - top, f = exp_of<true>(d);
         sum += parts[i].sum * (double)f;
         if (OP::kCentred) centred += (parts[i].centred + (float)parts[i].sum * d) * f;
     }
@@ -627,7 +641,7 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
             if (r.legal) bits &= legal_bits(r.legal + row * r.legal_stride, r.words, j);
             float x[V], unused = 0.0f;
             floats_of<true, T>(p, bits, x);
-            exponentials<false, V>(x, s.top, x, unused);
+            exponentials<false, false, V>(x, s.top, x, unused);
             write_vector<ONCE, T, OUT>(to, op.aligned, vec, head, r.actions, x, out.each, out.none, at, out.at_move);
         }
     }
@@ -660,17 +674,21 @@ __device__ __forceinline__ double block_sum(const float *values, int64_t n) {
     return s;
 }
 
+// The gradient's slope is known only when the last row of a pair has been read, so that logits are read twice: 9728 rows of
+// 32768 bf16 (638 MB) in 321 us, of which the first reading takes 109 us (5.8 TB/s) and this, which reads again and writes, 211 us
+// (6.0 TB/s).
+// Two and eight vectors a lane took a fifth longer than four.
 // A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.  Rows are taken from the last to the first: those that the
 // look at all rows has read last are in the cache still.
 template <bool ONCE, typename T>
-__global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces) {
+__global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces, int64_t first_block) {
     constexpr int V = Pack<T>::V, K = kGradientVectors;
     const int lane = threadIdx.x & 63;
-    if (blockIdx.x == 0) {
+    if (first_block + blockIdx.x == 0) {
         const double loss = block_sum<256>(p.pair_loss, p.pairs);
         if (threadIdx.x == 0) *p.loss = (float)loss;
     }
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), back = item / pieces;
+    const int64_t item = (first_block + blockIdx.x) * 4 + (threadIdx.x >> 6), back = item / pieces;
     if (back >= r.rows) return;
     const int64_t row = r.rows - 1 - back;
     const LineRows lines = line_rows(p, r.rows);
@@ -700,7 +718,7 @@ __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p,
         if (j >= r.actions) continue;
         float e[V], unused = 0.0f;
         floats_of<true, T>(x[k], bits[k], e);
-        exponentials<false, V>(e, top, e, unused);
+        exponentials<false, false, V>(e, top, e, unused);
         write_vector<ONCE, T, T>(to, aligned, vec, head, r.actions, e, each, slope == 0.0f, at, slope);
     }
 }
@@ -721,39 +739,57 @@ struct Launched {
     int64_t shares;
 };
 
-template <bool ONCE, typename T, int TEAM, int K, typename OP>
-static Launched run_narrow(const Rows &r, const OP &op, hipStream_t stream) {
-    const int64_t per_block = 256 / TEAM, blocks = (r.rows + per_block - 1) / per_block;
+// A launch's threads are counted in 32 bits: 2^21 blocks (of 1024 at most) at a time.
+constexpr int64_t kMostBlocks = 1 << 21;
+
+template <typename OP, typename LAUNCH>
+static Launched launch_rows(const Rows &r, const OP &op, int64_t per_block, const LAUNCH &launch) {
+    const int64_t blocks = (r.rows + per_block - 1) / per_block;
+    Rows some = r;
     OP o = op;
     if constexpr (OP::kLoss)
         if (blocks == 1) o.block_loss = op.p.loss;  // its share is the loss
-    k_narrow<ONCE, T, TEAM, K, OP><<<(unsigned)blocks, 256, 0, stream>>>(r, o);
-    return {hipGetLastError(), blocks};
+    hipError_t e = hipSuccess;
+    for (int64_t b = 0; b < blocks && e == hipSuccess; b += kMostBlocks) {
+        some.first = b * per_block;
+        launch(some, o, (unsigned)(blocks - b < kMostBlocks ? blocks - b : kMostBlocks));
+        e = hipGetLastError();
+        if constexpr (OP::kLoss) o.block_loss += kMostBlocks;
+    }
+    return {e, blocks};
+}
+
+template <bool ONCE, typename T, int TEAM, int K, typename OP>
+static Launched run_narrow(const Rows &r, const OP &op, hipStream_t stream) {
+    return launch_rows(r, op, 256 / TEAM, [&](const Rows &some, const OP &o, unsigned blocks) {
+        k_narrow<ONCE, T, TEAM, K, OP><<<blocks, 256, 0, stream>>>(some, o);
+    });
 }
 
 template <bool ONCE, typename T, int TEAM, int K, typename OP>
 static Launched run_rows(const Rows &r, const OP &op, hipStream_t stream) {
-    OP o = op;
-    if constexpr (OP::kLoss)
-        if (r.rows == 1) o.block_loss = op.p.loss;
-    k_rows<ONCE, T, TEAM, K, OP><<<(unsigned)r.rows, TEAM, 0, stream>>>(r, o);
-    return {hipGetLastError(), r.rows};
+    return launch_rows(r, op, 1, [&](const Rows &some, const OP &o, unsigned blocks) {
+        k_rows<ONCE, T, TEAM, K, OP><<<blocks, TEAM, 0, stream>>>(some, o);
+    });
 }
 
 template <bool ONCE, typename T, int BLOCK, typename OP>
 static Launched run_stream(const Rows &r, const OP &op, hipStream_t stream) {
-    k_stream<ONCE, T, BLOCK, OP><<<(unsigned)r.rows, BLOCK, 0, stream>>>(r, op);
-    return {hipGetLastError(), r.rows};
+    return launch_rows(r, op, 1, [&](const Rows &some, const OP &o, unsigned blocks) {
+        k_stream<ONCE, T, BLOCK, OP><<<blocks, BLOCK, 0, stream>>>(some, o);
+    });
 }
 
-// Wavefronts that fill the card: eight on each of 256 compute units.
+// Wavefronts that fill the card: eight on each of 256 compute units.  (Rows of 362 bf16 with their gradient: 4096 of them
+// take 6.7 us with 64 lanes each and 7.2 us with 16, 8192 10.7 and 8.4 us, 16384 17.1 and 13.2 us; 131072 83 and 59 us.)
 constexpr int64_t kFullOfRows = 256 * 8;
 
 template <bool ONCE, typename T, typename OP>
 static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_t stream) {
     const int64_t n = vectors_of<T>(r);
     // Few rows are done soonest with a lane for every vector; where the card is full of wavefronts all the same, many
-    // rows to a wavefront.
+    // rows to a wavefront: four vectors a lane and 16 lanes at least (with 8 a store's pieces are shorter than a cache
+    // line: 131072 rows of 225 floats took 74 us, with 16 lanes 62).
     if (n <= 256) {
         const auto full = [&](int team) { return r.rows >= kFullOfRows * (64 / team); };
         if (n <= 32 && full(16)) return run_narrow<ONCE, T, 16, 2>(r, op, stream);
@@ -773,14 +809,18 @@ static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_
         if constexpr (sizeof(T) == 4)
             if (n <= 16384) return run_rows<ONCE, T, 1024, 16>(r, op, stream);
     } else if (n <= 16384) {
-        return r.rows <= 256 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
+        // (2 waves of 256 compute units' blocks: 512 rows of 32768 bf16 take 14.2 us with blocks of 1024 and 15.8 us with
+        // blocks of 256, 64 rows 7.5 and 11.2 us, 1024 rows 22.1 and 18.2 us)
+        return r.rows <= 512 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
     }
     k_parts<ONCE, T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, op, w);
     k_apply<ONCE, T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, op, w);
     return {hipGetLastError(), r.rows};
 }
 
-// Logits that the second-level caches (4 MB on each of the card's eight dies) cannot hold together are not kept in them.
+// Logits that the second-level caches (4 MB on each of the card's eight dies) cannot hold together are not kept in them:
+// 8192 rows of 32768 bf16 take 204 us with nontemporal accesses and 229 us without, 131072 of 362 (95 MB) 60 and 71 us,
+// 32768 of 362 floats (47 MB) 26.8 and 26.5 us.
 static inline bool met_once(const Rows &r, int width) { return r.rows * (int64_t)r.actions * width > (int64_t)32 << 20; }
 
 template <typename T, typename OP>
@@ -830,13 +870,18 @@ Launched type_lines(const Rows &r, const PreferenceLoss &p, int64_t before, hipS
 template <typename T>
 hipError_t type_line_gradient(const Rows &r, const PreferenceLoss &p, hipStream_t stream) {
     const int64_t pieces = (vectors_of<T>(r) + 64 * kGradientVectors - 1) / (64 * kGradientVectors);
-    const dim3 grid((unsigned)((r.rows * pieces + 3) / 4));
+    const int64_t blocks = (r.rows * pieces + 3) / 4;
     const bool aligned = aligned_with<T>(r, p.grad, p.grad_stride);
-    if (met_once(r, sizeof(T)))
-        k_line_gradient<true, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces);
-    else
-        k_line_gradient<false, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces);
-    return hipGetLastError();
+    hipError_t e = hipSuccess;
+    for (int64_t b = 0; b < blocks && e == hipSuccess; b += kMostBlocks) {
+        const dim3 grid((unsigned)(blocks - b < kMostBlocks ? blocks - b : kMostBlocks));
+        if (met_once(r, sizeof(T)))
+            k_line_gradient<true, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces, b);
+        else
+            k_line_gradient<false, T><<<grid, 256, 0, stream>>>(r, p, aligned, (int)pieces, b);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 #define OMK_POLICY_TYPE(WORD, T)                                                                                         \

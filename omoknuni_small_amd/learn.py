@@ -4,6 +4,8 @@ From the network's logits to the priors of an expansion (Learner.priors, Batch.e
 search played to the gradient by the logits (Learner.policy_loss, Learner.preference_loss) and the step of the weights
 (AdamW).  All of it works on torch tensors that are on the learner's device, on the stream that is torch's current one
 there when a call is made, and waits for nothing.  Every call goes through libomk_forest.so; there is no host fallback.
+Import torch before anything here or in forest.py loads that library: the two then share one HIP runtime (a torch that brings its
+own and comes second finds no GPU; Learner says so).
 
 A gradient by the logits is handed on to the network that made them: `logits.backward(got.grad)`.
 """
@@ -138,10 +140,13 @@ class Learner:
     """
 
     def __init__(self, device=None):
-        self._lib = _library()
         self._h = C.c_void_p()
         import torch
+        self._lib = _library()
         self._torch = torch
+        if not torch.cuda.is_available():
+            raise OSError("torch finds no GPU: if there is one, import torch before the first Forest or Learner is made "
+                          "(a torch that brings a HIP runtime of its own has to be loaded first)")
         if device is None:
             device = torch.cuda.current_device()
         elif not isinstance(device, int):

@@ -240,8 +240,11 @@ def test_line_bounds_outside_the_rows(learner):
     got = learner.preference_loss(c.logits, c.d_moves, torch.tensor([-5, 20, 900], dtype=torch.int32, device="cuda"))
     want = learner.preference_loss(c.logits, c.d_moves, torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda"))
     assert torch.equal(got.logprob, want.logprob) and torch.equal(got.grad, want.grad) and torch.equal(got.loss, want.loss)
-    got = learner.preference_loss(c.logits, c.d_moves, torch.tensor([40, 20, 2 ** 31 - 1], dtype=torch.int32, device="cuda"), grad=False)
-    assert got.logprob[0] == 0 and got.logprob[1] < 0
+    got = learner.preference_loss(c.logits, c.d_moves, torch.tensor([40, 20, 2 ** 31 - 1], dtype=torch.int32, device="cuda"))
+    want = learner.preference_loss(c.logits, c.d_moves, torch.tensor([40, 40, 50], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got.logprob, want.logprob) and torch.equal(got.grad, want.grad)
+    got = learner.preference_loss(c.logits, c.d_moves, torch.tensor([40, 45, 20], dtype=torch.int32, device="cuda"))
+    assert got.logprob.tolist() == [0, 0] and (got.grad == 0).all()
 
 
 def test_many_pairs_and_long_lines(learner):
@@ -315,6 +318,37 @@ def test_rows_far_apart(learner):
     far.copy_(c.logits)
     c.logits = far
     policy_case(learner, c, grad=far)
+
+
+@pytest.mark.parametrize("rows,actions", [((1 << 21) * 16 + 5, 3), ((1 << 21) + 3, 4100)])
+def test_more_rows_than_a_launch_takes(learner, rows, actions):
+    """What the first and the last rows come to where a launch's blocks do not reach the end, by the same rows alone."""
+    gen = torch.Generator("cuda").manual_seed(1)
+    x = torch.empty(rows, actions, dtype=torch.float16, device="cuda")
+    for at in range(0, rows, 1 << 19):
+        x[at:at + (1 << 19)].normal_(0, 2, generator=gen)
+    moves = torch.randint(0, actions, (rows,), device="cuda", generator=gen, dtype=torch.int32)
+    adv = torch.randn(rows, device="cuda", generator=gen)
+    ends = [slice(0, 64), slice(rows - 64, rows)]
+    few = torch.cat([x[e] for e in ends]).clone()
+    fewer = torch.cat([moves[e] for e in ends])
+    lp = learner.logprobs(x, moves, entropy=True)
+    alone = learner.logprobs(few, fewer, entropy=True)
+    # (a row alone is summed in another order: two roundings of a sum whose terms are as many as the actions)
+    for a, b in zip(lp, alone):
+        assert (torch.cat([a[e] for e in ends]) - b).abs().max() <= (actions / 64 + 64) * O.U * 4
+    begin = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device="cuda")
+    lines = learner.preference_loss(x, moves, begin, beta=1e-9, grad=False)
+    sums = torch.stack([lp.logprob[:rows // 2].double().sum(), lp.logprob[rows // 2:].double().sum()])
+    assert ((lines.logprob.double() - sums).abs() <= sums.abs() * 4 * O.U).all()
+    got = learner.policy_loss(x, moves, lp.logprob, adv, scale=1.0, grad=x)  # in place: the last use of these logits
+    assert (got.logprob - lp.logprob).abs().max() <= (actions / 64 + 64) * O.U * 4
+    want = learner.policy_loss(few, fewer, torch.cat([lp.logprob[e] for e in ends]), torch.cat([adv[e] for e in ends]), scale=1.0)
+    # nearly the same numbers, each rounded to 11 bits: a step of these apart at most
+    assert ((torch.cat([x[e] for e in ends]).double() - want.grad.double()).abs() <=
+            2.0 ** -24 + want.grad.double().abs() * (2.0 ** -10 + 2.0 ** -18)).all()
+    # the ratios are 1 within the log-probabilities' rounding, so the loss is minus the advantages' sum
+    assert abs(float(got.loss) + float(adv.double().sum())) <= float(adv.double().abs().sum()) * ((actions / 64 + 64) * O.U * 4 + 2.0 ** -22)
 
 
 def test_graphs_and_streams(learner):

@@ -135,7 +135,7 @@ def test_preference_loss_refuses(handle):
     for change in (dict(d_loss=None), dict(grad_stride=3), dict(d_grad=address(0) + 4), dict(d_margin=address(8) + 1)):
         assert preference(handle, out=change) == INVALID, change
     assert preference(handle, pairs=-1) == INVALID
-    assert preference(handle, pairs=1 << 31) == INVALID
+    assert preference(handle, pairs=(1 << 23) + 1) == INVALID
     assert preference(handle, d_moves=None) == INVALID
     assert preference(handle, d_begin=None) == INVALID
     assert preference(handle, d_begin=address(6) + 1) == INVALID
@@ -168,6 +168,9 @@ def test_adamw_refuses(handle):
         assert adamw(handle, **change) == INVALID, change
     for change in (dict(d_m_scale=None), dict(d_v_scale=None), dict(d_v_scale=address(4) + 2)):
         assert adamw(handle, tensor=change, state_type=3) == INVALID, change
+    for change in (dict(d_m=address(0) + 4 * 299), dict(d_v=address(1)), dict(d_v=address(1) - 4 * 299)):
+        assert adamw(handle, tensor=change) == INVALID and "overlap" in message(), change
+    assert adamw(handle, tensor=dict(d_v_scale=address(3) + 4), state_type=3) == INVALID and "overlap" in message()
     assert adamw(handle, param_type=1, grad_type=2) == UNSUPPORTED
     assert adamw(handle, tensor=dict(d_copy=address(9)), param_type=1, grad_type=1, copy_type=1) == UNSUPPORTED
     assert adamw(None) == INVALID
@@ -181,6 +184,16 @@ def test_a_learner_needs_a_device():
     assert lib.omk_learner_create(0, None) == INVALID
     assert lib.omk_learner_set_stream(None, None) == INVALID
     assert lib.omk_learner_destroy(None) == 0 and lib.omk_adamw_destroy(None) == 0
+
+
+def test_torch_without_a_gpu_is_named():
+    import torch
+
+    import omoknuni_small_amd as omk
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is here")
+    with pytest.raises(OSError, match="import torch before"):
+        omk.Learner()
 
 
 def test_masks_of_move_lists():
