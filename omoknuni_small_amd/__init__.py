@@ -2,6 +2,6 @@
 virtual loss, value backup and leaf gather behind a C ABI (include/omk_forest.h), and what lies
 between the search and its network: priors, policy losses and AdamW (include/omk_learn.h)."""
 from .forest import Forest, Batch, TranspositionTable, SelectParams, OmkError, library_path, load_library, compact_legal  # noqa: F401
-from .learn import Learner, AdamW, pack_legal  # noqa: F401
+from .learn import Learner, AdamW, pack_legal, legal_of_moves  # noqa: F401
 
-__all__ = ["Learner", "AdamW", "pack_legal", "Forest", "Batch", "TranspositionTable", "SelectParams", "OmkError", "library_path", "load_library", "compact_legal"]
+__all__ = ["Learner", "AdamW", "pack_legal", "legal_of_moves", "Forest", "Batch", "TranspositionTable", "SelectParams", "OmkError", "library_path", "load_library", "compact_legal"]
