@@ -87,7 +87,9 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
  *   l     = -min(ratio * advantage, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantage)
  *           + kl_weight * kl,   kl = exp(ref_logprob - lp) - (ref_logprob - lp) - 1
  *   loss  = scale * sum over rows of weight * l
- * and the gradient of the loss by every logit.  An advantage of 0 gives no loss at whatever ratio. */
+ * and the gradient of the loss by every logit.  An advantage of 0 gives no loss at whatever ratio, and a row of weight 0
+ * adds nothing to loss and gradient, whatever its other columns hold.  Results of a row each (d_logprob, d_kl) must not
+ * overlap what is read. */
 typedef struct omk_policy_samples {
     const int32_t *d_moves;
     const float *d_old_logprob;
@@ -119,7 +121,7 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
  * count nothing) and u_k = beta * ((S_2k - ref_2k) - (S_2k+1 - ref_2k+1)):
  *   loss = scale * sum over pairs of -(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)
  * d_ref_logprob[s] = the line's sum under the reference policy (NULL: 0); a call without d_grad on the reference's logits
- * gives it as d_line_logprob.  d_line_begin must not decrease.  (Bounds that do not fit are taken as the nearest that
+ * gives it as d_line_logprob (which must not overlap it).  d_line_begin must not decrease.  (Bounds that do not fit are taken as the nearest that
  * do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
  * empty; which line's gradient a row of two lines gets is open.)  Rows before the first line and behind the last are not
  * read.  0 .. OMK_MAX_PAIRS pairs. */

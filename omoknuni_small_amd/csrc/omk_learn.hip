@@ -239,6 +239,11 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
         if (out->d_grad)
             if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
                 return rc;
+        const void *results[] = {out->d_logprob, out->d_kl};
+        for (const void *to : results)
+            for (int i = 0; i < 5; i++)  // (the columns that are read come first in `all`)
+                if (to && all[i] && overlap(to, r.rows * 4, all[i], r.rows * 4))
+                    return learn_fail(OMK_ERR_INVALID, "%s: a result lies across what is read", who);
         if (int rc = check_work(who, d_work, work_bytes, omk_policy_loss_work(r.rows, r.actions))) return rc;
     }
     OnDevice on(l->device);
@@ -299,6 +304,14 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
         if (r.rows && out->d_grad)
             if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
                 return rc;
+        const struct {
+            const void *to;
+            int64_t bytes;
+        } results[] = {{out->d_margin, pairs * 4}, {out->d_line_logprob, pairs * 8}};
+        for (const auto &x : results)
+            if (x.to && ((d_ref_logprob && overlap(x.to, x.bytes, d_ref_logprob, pairs * 8)) ||
+                         overlap(x.to, x.bytes, d_line_begin, pairs * 8 + 4)))
+                return learn_fail(OMK_ERR_INVALID, "%s: a result lies across what is read", who);
         if (int rc = check_work(who, d_work, work_bytes, omk_preference_loss_work(r.rows, r.actions, pairs))) return rc;
     }
     OnDevice on(l->device);

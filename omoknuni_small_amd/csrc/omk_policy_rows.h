@@ -233,12 +233,14 @@ struct PolicyOp {
             if (p.ref_logprob) {
                 const float d = (float)((double)p.ref_logprob[row] - exact);
                 kl = exp_minus_linear(d);
-                loss += p.kl_weight * kl;
-                slope -= p.kl_weight * (d + kl);
+                if (p.kl_weight > 0.0f) {  // (a divergence that is only reported may be infinite)
+                    loss += p.kl_weight * kl;
+                    slope -= p.kl_weight * (d + kl);
+                }
             }
             const float w = (p.weight ? p.weight[row] : 1.0f) * p.scale;
-            loss *= w;
-            slope *= w;
+            loss = w == 0.0f ? 0.0f : loss * w;
+            slope = w == 0.0f ? 0.0f : slope * w;
         }
         if (writes) {
             p.logprob[row] = lp;

@@ -192,6 +192,25 @@ def test_numbers_that_are_none(learner, actions):
     assert got.grad.isnan().any(1).tolist() == [False, False, True, False, False, False]
 
 
+@pytest.mark.parametrize("actions", [300, 3000, 70000])
+def test_rows_of_weight_0_and_a_divergence_that_is_only_reported(learner, actions):
+    x = torch.randn(9, actions, device="cuda")
+    moves = torch.arange(9, dtype=torch.int32, device="cuda")
+    lp = learner.logprobs(x, moves).logprob
+    adv, weight, ref = torch.ones(9, device="cuda"), torch.ones(9, device="cuda"), lp.clone()
+    old = lp.clone()
+    weight[4], old[4], adv[5], weight[5], ref[6], weight[6] = 0, math.nan, math.inf, 0, math.inf, 0
+    got = learner.policy_loss(x, moves, old, adv, ref_logprob=ref, weight=weight, kl_weight=0.5)
+    rest = [0, 1, 2, 3, 7, 8]
+    want = learner.policy_loss(x[rest], moves[rest], lp[rest], adv[rest], ref_logprob=lp[rest], kl_weight=0.5, scale=1 / 9)
+    assert (got.grad[4:7] == 0).all() and torch.equal(got.grad[rest], want.grad)
+    assert abs(float(got.loss - want.loss)) <= 4 * O.U
+    # a reference that gives a move all but no chance: its divergence passes the largest float, and is weighed with 0
+    ref = lp + 100.0
+    got = learner.policy_loss(x, moves, lp, torch.ones(9, device="cuda"), ref_logprob=ref)
+    assert got.kl.isinf().all() and got.loss.isfinite() and got.grad.isfinite().all()
+
+
 def preference_case(learner, c, lengths, beta=0.3, smoothing=0.1, before=0, use_ref=True, grad=True):
     begin = before + np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
     lp, counts, _ = c.oracle.taken(c.moves)

@@ -91,6 +91,9 @@ def test_policy_loss_refuses(handle):
                    dict(d_kl=address(8) + 2), dict(grad_stride=1 << 61),
                    dict(d_grad=address(0) + 2), dict(d_grad=address(0), grad_stride=226)):
         assert policy(handle, out=change) == INVALID, change
+    for n in (5, 6, 7, 8):
+        assert policy(handle, out=dict(d_logprob=address(n) + 4 * 7)) == INVALID and "across" in message()
+        assert policy(handle, out=dict(d_kl=address(n) - 4 * 7)) == INVALID and "across" in message()
     needed = learn._library().omk_policy_loss_work(8, 225)
     assert needed > 0
     assert policy(handle, work=needed - 1) == CAPACITY
@@ -134,6 +137,8 @@ def test_preference_loss_refuses(handle):
         assert preference(handle, params=change) == INVALID, change
     for change in (dict(d_loss=None), dict(grad_stride=3), dict(d_grad=address(0) + 4), dict(d_margin=address(8) + 1)):
         assert preference(handle, out=change) == INVALID, change
+    for change in (dict(d_margin=address(6) + 4), dict(d_line_logprob=address(6) + 24), dict(d_margin=address(6) - 8)):
+        assert preference(handle, out=change) == INVALID and "across" in message(), change
     assert preference(handle, pairs=-1) == INVALID
     assert preference(handle, pairs=(1 << 23) + 1) == INVALID
     assert preference(handle, d_moves=None) == INVALID
