@@ -9,8 +9,10 @@ own and comes second finds no GPU; Learner says so).
 
 A gradient by the logits is handed on to the network that made them: `logits.backward(got.grad)`.
 """
+import array
 import collections
 import ctypes as C
+import operator
 
 import numpy as np
 
@@ -76,6 +78,7 @@ _ARGTYPES = {
     "omk_adamw_set_steps": (_VP, _I64), "omk_adamw_get_steps": (_VP, _VP),
 }
 _ready = None
+_DTYPE = operator.attrgetter("dtype")
 _F32, _BF16, _F16, _F8, _NONE = 0, 1, 2, 3, -1
 
 
@@ -224,7 +227,7 @@ class Learner:
 
     def _gradient(self, grad, logits):
         if grad is True:
-            return self._empty(logits.shape, dtype=logits.dtype, device=self._place)
+            return logits.new_empty(logits.shape)
         if grad is None or grad is False:
             return None
         self._same_place("grad", grad, logits.dtype)
@@ -291,7 +294,7 @@ class Learner:
         need = self._lib.omk_policy_loss_work(rows, actions)
         # one allocation for what is small: log-probabilities, kl, the loss, and the work space behind them
         behind = (2 * rows + 4) // 4 * 4
-        small = self._empty(behind + (need + 3) // 4, dtype=f32, device=self._place)
+        small = old_logprob.new_empty(behind + (need + 3) // 4)
         at = small.data_ptr()
         out = _PolicyOut(at + 8 * rows, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                          at + 4 * rows)
@@ -398,7 +401,6 @@ class AdamW:
                          _NONE if copy_type is None else kinds[copy_type], _F32 if states == "f32" else _F8,
                          float(betas[0]), float(betas[1]), float(eps), int(seed) & 0xFFFFFFFF)
         self._sizes = [p.numel() for p in self.params]
-        self._grads = C.c_void_p * n
         learner._on_stream()
         _check(self._lib.omk_adamw_create(learner._h, C.byref(desc), C.byref(self._h)))
 
@@ -420,15 +422,23 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError("%d gradients of %d parameters" % (len(grads), len(self.params)))
         learner, dtype, device = self.learner, self.grad_type, self.learner.device
-        at = []
-        for g, n in zip(grads, self._sizes):
-            if g is None:
-                at.append(None)
-            elif g.dtype is dtype and g.numel() == n and g.get_device() == device and g.is_contiguous():
-                at.append(g.data_ptr())
-            else:
-                raise ValueError("gradient %d: %s %s on %s: %d contiguous values of %s on device %d are wanted" %
-                                 (len(at), g.dtype, tuple(g.shape), g.device, n, dtype, device))
+        T = learner._torch.Tensor
+        at = None
+        if not any(g is None for g in grads):
+            # (a look at all tensors' sizes, then at all their devices, .. takes half of what a look at tensor after tensor does)
+            if (list(map(T.numel, grads)) == self._sizes and set(map(T.get_device, grads)) == {device} and
+                    all(map(T.is_contiguous, grads)) and set(map(_DTYPE, grads)) == {dtype}):
+                at = list(map(T.data_ptr, grads))
+        if at is None:
+            at = []
+            for g, n in zip(grads, self._sizes):
+                if g is None:
+                    at.append(0)
+                elif g.dtype is dtype and g.numel() == n and g.get_device() == device and g.is_contiguous():
+                    at.append(g.data_ptr())
+                else:
+                    raise ValueError("gradient %d: %s %s on %s: %d contiguous values of %s on device %d are wanted" %
+                                     (len(at), g.dtype, tuple(g.shape), g.device, n, dtype, device))
         d_lr, number = None, 0.0
         if isinstance(lr, (int, float)):
             number = lr
@@ -436,7 +446,8 @@ class AdamW:
             d_lr = learner._vector("lr", lr.reshape(-1), 1, learner._f32)
         d_scale = None if grad_scale is None else learner._vector("grad_scale", grad_scale.reshape(-1), 1, learner._f32)
         learner._on_stream()
-        _check(self._lib.omk_adamw_step(self._h, self._grads(*at), number, d_lr, d_scale))
+        addresses = array.array("Q", at)
+        _check(self._lib.omk_adamw_step(self._h, addresses.buffer_info()[0], number, d_lr, d_scale))
 
     def state(self):
         """The moments, as they are held: dict(m, v) and with 8-bit states (float8_e4m3fn, v's square root) m_scale and
