@@ -121,8 +121,8 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
  * count nothing) and u_k = beta * ((S_2k - ref_2k) - (S_2k+1 - ref_2k+1)):
  *   loss = scale * sum over pairs of -(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)
  * d_ref_logprob[s] = the line's sum under the reference policy (NULL: 0); a call without d_grad on the reference's logits
- * gives it as d_line_logprob (which must not overlap it).  d_line_begin must not decrease.  (Bounds that do not fit are taken as the nearest that
- * do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
+ * gives it as d_line_logprob (which must not overlap it).  d_line_begin must not decrease.  (Bounds that do not fit
+ * are taken as the nearest that do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
  * empty; which line's gradient a row of two lines gets is open.)  Rows before the first line and behind the last are not
  * read.  0 .. OMK_MAX_PAIRS pairs. */
 typedef struct omk_preference_params {

@@ -444,7 +444,8 @@ int omk_adamw_create(omk_learner *l, const omk_adamw_desc *desc, omk_adamw **out
     o->first_chunk.swap(first_chunk);
     o->elements.swap(elements);
     OnDevice on(l->device);
-    const size_t at_done = 256, at_tensors = at_done + kCountGroups * kCountStep * 4, at_chunks = at_tensors + (tensors.size() * sizeof(AdamTensor) + 255) / 256 * 256;
+    const size_t at_done = 256, at_tensors = at_done + kCountGroups * kCountStep * 4;
+    const size_t at_chunks = at_tensors + (tensors.size() * sizeof(AdamTensor) + 255) / 256 * 256;
     hipError_t e = on.status;
     if (e == hipSuccess) e = hipMalloc((void **)&o->memory, at_chunks + chunks.size() * sizeof(AdamChunk) + 16);
     if (e == hipSuccess) {

@@ -27,7 +27,7 @@ __device__ __forceinline__ double log_of_sum(double s) {
         k--;
     }
     const float near = (float)f;
-    return (double)k * kLn2 + (double)(logf(near) + (float)(f - (double)near) / near);
+    return (double)k * kLn2 + (double)(logf(near) + (float)(f - (double)near) * __builtin_amdgcn_rcpf(near));
 }
 
 // ---- 16 bytes of a row ----
@@ -246,7 +246,7 @@ struct PolicyOp {
             p.logprob[row] = lp;
             if (p.kl) p.kl[row] = kl;
         }
-        return {slope == 0.0f ? 0.0f : -slope / (float)s.sum, slope, m.move, slope == 0.0f, loss};
+        return {slope == 0.0f ? 0.0f : -slope * __builtin_amdgcn_rcpf((float)s.sum), slope, m.move, slope == 0.0f, loss};
     }
 };
 
@@ -680,7 +680,8 @@ __device__ __forceinline__ double block_sum(const float *values, int64_t n) {
 // 32768 bf16 (638 MB) in 321 us, of which the first reading takes 109 us (5.8 TB/s) and this, which reads again and writes, 211 us
 // (6.0 TB/s).
 // Two and eight vectors a lane took a fifth longer than four.
-// A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.  Rows are taken from the last to the first: those that the
+// A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.
+// Rows are taken from the last to the first: those that the
 // look at all rows has read last are in the cache still.
 template <bool ONCE, typename T>
 __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p, bool aligned, int pieces, int64_t first_block) {

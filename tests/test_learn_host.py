@@ -5,6 +5,7 @@ import ctypes as C
 import math
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -22,6 +23,21 @@ def test_header_library_and_mirror_agree():
     assert declared == sorted(learn.EXPORTS) == sorted(learn._ARGTYPES)
     for name in declared:
         assert hasattr(lib, name)
+
+
+def test_header_is_c(tmp_path):
+    """Both headers as C, and the structures as the mirror lays them out."""
+    structs = [("omk_policy_rows", learn._Rows), ("omk_policy_samples", learn._Samples), ("omk_policy_loss_params", learn._PolicyParams),
+               ("omk_policy_loss_out", learn._PolicyOut), ("omk_preference_params", learn._PreferenceParams),
+               ("omk_preference_out", learn._PreferenceOut), ("omk_adamw_tensor", learn._AdamTensor), ("omk_adamw_desc", learn._AdamDesc)]
+    lines = ["#include <stddef.h>", '#include "omk_learn.h"']
+    for name, mirror in structs:
+        names = [f[0] for f in mirror._fields_]
+        lines.append("_Static_assert(sizeof(%s) == %d, \"%s\");" % (name, C.sizeof(mirror), name))
+        lines += ["_Static_assert(offsetof(%s, %s) == %d, \"%s.%s\");" % (name, f, getattr(mirror, f).offset, name, f) for f in names]
+    source = tmp_path / "header.c"
+    source.write_text("\n".join(lines) + "\nint main(void) { return 0; }\n")
+    subprocess.check_call(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(source)])
 
 
 @pytest.fixture
