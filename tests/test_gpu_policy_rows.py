@@ -141,6 +141,29 @@ def test_policy_loss(learner, rows, actions, kind, legal):
     policy_case(learner, c, use_ref=actions % 2 == 1, use_weight=rows % 2 == 1)
 
 
+@pytest.mark.parametrize("kind,actions", [("f32", 4), ("f32", 33), ("f32", 101), ("f32", 225), ("f32", 256), ("f32", 499),
+                                          ("bf16", 7), ("bf16", 8), ("bf16", 9), ("bf16", 225), ("f16", 362), ("bf16", 504), ("f16", 999)])
+@pytest.mark.parametrize("layout", ["together", "apart", "in place", "shifted"])
+def test_many_narrow_rows(learner, kind, actions, layout):
+    """As many rows as are taken several to a wavefront, where the end of one and the beginning of the next share 16 bytes:
+    rows that follow one another, rows with a gap, gradients in the logits' place and ones whose vectors lie
+    elsewhere."""
+    rows = 8192 + 37
+    c = Case(actions, rows, actions, kind, 0.5 if layout != "apart" else None, stride=3 if layout == "apart" else 0)
+    near(learner.priors(c.logits, legal=c.legal), c.oracle.p, c.oracle.priors_off(), "priors")
+    got = learner.logprobs(c.logits, c.d_moves, legal=c.legal, entropy=True)
+    near(got.entropy, c.oracle.entropy, c.oracle.entropy_off(), "entropy")
+    grad = True
+    if layout == "in place":
+        grad = c.logits
+    elif layout == "shifted":
+        out = torch.full((rows * actions + 9,), 9.0, dtype=TYPES[kind], device="cuda")
+        grad = out[1:1 + rows * actions].view(rows, actions)
+    policy_case(learner, c, grad=grad)
+    if layout == "shifted":
+        assert out[0] == 9 and (out[1 + rows * actions:] == 9).all()
+
+
 @pytest.mark.parametrize("clip_low,clip_high,kl_weight", [(0.0, 0.0, 0.0), (1.0, 4.0, 1.0), (2.5, 0.1, 0.0)])
 def test_policy_loss_borders(learner, clip_low, clip_high, kl_weight):
     policy_case(learner, Case(5, 200, 225, "f32", 0.4), clip_low, clip_high, kl_weight)
