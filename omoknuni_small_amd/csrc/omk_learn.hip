@@ -213,7 +213,7 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
 }
 
 int64_t omk_policy_loss_work(int64_t rows, int32_t actions) {
-    return rows > 0 ? (rows * 4 + 15) / 16 * 16 + wide_work(rows, actions) : 0;
+    return rows > 0 ? (rows * 8 + 15) / 16 * 16 + wide_work(rows, actions) : 0;
 }
 
 int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_policy_samples *samples,
@@ -260,15 +260,15 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
     p.weight = samples->d_weight;
     p.log_low = params->clip_low < 1.0 ? std::log(1.0 - params->clip_low) : -INFINITY;
     p.log_high = std::log(1.0 + params->clip_high);
-    p.low = (float)(1.0 - params->clip_low);
-    p.high = (float)(1.0 + params->clip_high);
-    p.kl_weight = (float)params->kl_weight;
-    p.scale = (float)params->scale;
+    p.low = 1.0 - params->clip_low;
+    p.high = 1.0 + params->clip_high;
+    p.kl_weight = params->kl_weight;
+    p.scale = params->scale;
     p.grad = out->d_grad;
     p.grad_stride = out->grad_stride;
     p.logprob = out->d_logprob;
     p.kl = out->d_kl;
-    p.shares = (float *)d_work;
+    p.shares = (double *)d_work;
     p.loss = out->d_loss;
     LEARN_TRY(launch_policy_loss(rows->type, r, p, l->stream));
     return OMK_OK;

@@ -33,12 +33,12 @@ struct PolicyLoss {
     const int32_t *moves;
     const float *old_logprob, *advantage, *ref_logprob, *weight;
     double log_low, log_high;  // borders of the ratio's logarithm
-    float low, high;           // borders of the ratio
-    float kl_weight, scale;
+    double low, high;          // borders of the ratio
+    double kl_weight, scale;
     void *grad;
     int64_t grad_stride;
     float *logprob, *kl;
-    float *shares;  // work space: the blocks' shares of the loss (at most one a row), and what wide rows need
+    double *shares;  // work space: the blocks' shares of the loss (at most one a row), and what wide rows need
     float *loss;
 };
 

@@ -9,7 +9,8 @@ OMK_POLICY_TYPE(extern, f16_t)
 
 constexpr int kSumBlock = 1024;
 
-__global__ __launch_bounds__(kSumBlock) void k_sum(const float *values, int64_t n, float *out) {
+template <typename F>
+__global__ __launch_bounds__(kSumBlock) void k_sum(const F *values, int64_t n, float *out) {
     const double s = block_sum<kSumBlock>(values, n);
     if (threadIdx.x == 0) *out = (float)s;
 }

@@ -17,19 +17,6 @@ struct RowStats {
     double sum;
 };
 
-// log(s) in 64 bits: the exponent is taken off, so that what is rounded is the logarithm of a number near 1.  (A loss
-// compares a ratio with borders: the log-probability keeps more than the 24 bits of a float.)
-__device__ __forceinline__ double log_of_sum(double s) {
-    int k = __builtin_amdgcn_frexp_exp(s);
-    double f = __builtin_amdgcn_frexp_mant(s);  // [0.5, 1)
-    if (f < 0.70710678) {
-        f *= 2.0;
-        k--;
-    }
-    const float near = (float)f;
-    return (double)k * kLn2 + (double)(logf(near) + (float)(f - (double)near) * __builtin_amdgcn_rcpf(near));
-}
-
 // ---- 16 bytes of a row ----
 
 // Vectors of a row lie at multiples of 16 bytes of the matrix, not of the row: the first holds `head` elements of what
@@ -150,7 +137,7 @@ struct RowOut {
     float each, at_move;
     int32_t move;
     bool none;
-    float share;  // of the loss
+    double share;  // of the loss
 };
 
 struct PriorsOp {
@@ -158,7 +145,7 @@ struct PriorsOp {
     template <typename T>
     using Element = float;
     const int32_t *moves;  // nullptr
-    float *block_loss;     // nullptr
+    double *block_loss;    // nullptr
     float *priors;
     int64_t stride;
     bool aligned;
@@ -175,12 +162,12 @@ struct PriorsOp {
 struct LogprobsOp {
     static constexpr bool kCentred = true, kElements = false, kMoves = true, kLoss = false;
     const int32_t *moves;
-    float *block_loss;  // nullptr
+    double *block_loss;  // nullptr
     float *logprob, *entropy;
     __device__ bool skips(const Rows &, int64_t) const { return false; }
     __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
         if (writes) {
-            const double log_sum = log_of_sum(s.sum);
+            const double log_sum = log(s.sum);
             if (entropy) entropy[row] = s.sum == 0.0 ? 0.0f : (float)(log_sum - (double)(s.centred / (float)s.sum));
             if (logprob)
                 logprob[row] = m.move < 0       ? 0.0f
@@ -210,43 +197,53 @@ struct PolicyOp {
     template <typename T>
     using Element = T;
     const int32_t *moves;
-    float *block_loss;  // a block's share of the loss, by the block's number (by the row where rows are cut)
+    double *block_loss;  // a block's share of the loss, by the block's number (by the row where rows are cut)
     PolicyLoss p;
     bool aligned;
     __device__ bool skips(const Rows &, int64_t) const { return false; }
+    __device__ void add(int64_t block, double share) const {
+        if (block_loss)
+            block_loss[block] = share;
+        else
+            *p.loss = (float)share;
+    }
     template <typename OUT>
     __device__ OUT *elements(int64_t row) const {
         return p.grad ? (OUT *)p.grad + row * p.grad_stride : nullptr;
     }
     __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
-        float lp = 0.0f, kl = 0.0f, loss = 0.0f, slope = 0.0f;
+        // (in 64 bits up to the sum: advantages have a mean of about 0, and what is left of a sum of rows is small beside them)
+        double loss = 0.0, slope = 0.0;
+        float lp = 0.0f, kl = 0.0f;
         if (m.chosen != -INFINITY) {
-            const double exact = (double)m.chosen - (double)s.top - log_of_sum(s.sum);
+            const double exact = (double)m.chosen - (double)s.top - log(s.sum);
             lp = (float)exact;
             const float a = p.advantage[row];
             const double shift = exact - (double)p.old_logprob[row];
             if (a > 0.0f ? shift > p.log_high : a < 0.0f && shift < p.log_low) {
-                loss = -(a > 0.0f ? p.high : p.low) * a;
+                loss = -(a > 0.0f ? p.high : p.low) * (double)a;
             } else if (a != 0.0f) {
-                loss = slope = -expf((float)shift) * a;
+                loss = slope = -exp(shift) * (double)a;
             }
             if (p.ref_logprob) {
                 const float d = (float)((double)p.ref_logprob[row] - exact);
                 kl = exp_minus_linear(d);
-                if (p.kl_weight > 0.0f) {  // (a divergence that is only reported may be infinite)
-                    loss += p.kl_weight * kl;
-                    slope -= p.kl_weight * (d + kl);
+                if (p.kl_weight > 0.0) {  // (a divergence that is only reported may be infinite)
+                    loss += p.kl_weight * (double)kl;
+                    slope -= p.kl_weight * ((double)d + (double)kl);
                 }
             }
-            const float w = (p.weight ? p.weight[row] : 1.0f) * p.scale;
-            loss = w == 0.0f ? 0.0f : loss * w;
-            slope = w == 0.0f ? 0.0f : slope * w;
+            const double w = (p.weight ? (double)p.weight[row] : 1.0) * p.scale;
+            loss = w == 0.0 ? 0.0 : loss * w;
+            slope = w == 0.0 ? 0.0 : slope * w;
         }
         if (writes) {
             p.logprob[row] = lp;
             if (p.kl) p.kl[row] = kl;
         }
-        return {slope == 0.0f ? 0.0f : -slope * __builtin_amdgcn_rcpf((float)s.sum), slope, m.move, slope == 0.0f, loss};
+        const float by_logprob = (float)slope;
+        return {by_logprob == 0.0f ? 0.0f : -by_logprob * __builtin_amdgcn_rcpf((float)s.sum), by_logprob, m.move,
+                by_logprob == 0.0f, loss};
     }
 };
 
@@ -264,7 +261,7 @@ __device__ __forceinline__ LineRows line_rows(const PreferenceLoss &p, int64_t r
 struct LineOp {
     static constexpr bool kCentred = false, kElements = false, kMoves = true, kLoss = false;
     const int32_t *moves;
-    float *block_loss;  // nullptr
+    double *block_loss;  // nullptr
     PreferenceLoss p;
     __device__ bool skips(const Rows &r, int64_t row) const {
         const LineRows lines = line_rows(p, r.rows);
@@ -275,7 +272,7 @@ struct LineOp {
             const bool counts = m.chosen != -INFINITY;
             p.top[row] = s.top;
             p.inverse[row] = counts ? 1.0f / (float)s.sum : 0.0f;
-            p.logprob[row] = counts ? (double)m.chosen - (double)s.top - log_of_sum(s.sum) : 0.0;
+            p.logprob[row] = counts ? (double)m.chosen - (double)s.top - log(s.sum) : 0.0;
             p.slope[row] = 0.0f;  // until its line says otherwise
         }
         return {0.0f, 0.0f, -1, true, 0.0f};
@@ -420,10 +417,10 @@ __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
     }
     if constexpr (OP::kLoss) {
         __shared__ double shares[4];
-        const double share = team_sum<64>((double)out.share);
+        const double share = team_sum<64>(out.share);
         if ((threadIdx.x & 63) == 0) shares[threadIdx.x >> 6] = share;
         __syncthreads();
-        if (threadIdx.x == 0) op.block_loss[blockIdx.x] = (float)(shares[0] + shares[1] + (shares[2] + shares[3]));
+        if (threadIdx.x == 0) op.add(blockIdx.x, shares[0] + shares[1] + (shares[2] + shares[3]));
     }
 }
 
@@ -504,7 +501,8 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
             }
         }
     }
-    if (OP::kLoss && threadIdx.x == 0) op.block_loss[blockIdx.x] = shared_out.share;
+    if constexpr (OP::kLoss)
+        if (threadIdx.x == 0) op.add(blockIdx.x, shared_out.share);
 }
 
 // ---- rows of which nothing but numbers is wanted ----
@@ -622,7 +620,8 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
         const RowOut o = op.row(row, s, m, piece == 0 && threadIdx.x == 0);
         if (threadIdx.x == 0) {
             shared_out = o;
-            if (OP::kLoss && piece == 0) op.block_loss[row] = o.share;
+            if constexpr (OP::kLoss)
+                if (piece == 0) op.add(row, o.share);
         }
     }
     if constexpr (OP::kElements) {
@@ -654,14 +653,14 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
 constexpr int kGradientVectors = 4;  // of a lane
 
 // The sum of n values by one block, in one order whatever runs beside it: in its first thread.
-template <int BLOCK>
-__device__ __forceinline__ double block_sum(const float *values, int64_t n) {
+template <int BLOCK, typename F>
+__device__ __forceinline__ double block_sum(const F *values, int64_t n) {
     __shared__ double part[BLOCK / 64];
     double s = 0.0;
     // (eight at a time, so that as many loads are on their way)
     int64_t i = threadIdx.x;
     for (; i + 7 * BLOCK < n; i += 8 * BLOCK) {
-        float v[8];
+        F v[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) v[k] = values[i + k * BLOCK];
 #pragma unroll
@@ -751,13 +750,14 @@ static Launched launch_rows(const Rows &r, const OP &op, int64_t per_block, cons
     Rows some = r;
     OP o = op;
     if constexpr (OP::kLoss)
-        if (blocks == 1) o.block_loss = op.p.loss;  // its share is the loss
+        if (blocks == 1) o.block_loss = nullptr;  // its share is the loss
     hipError_t e = hipSuccess;
     for (int64_t b = 0; b < blocks && e == hipSuccess; b += kMostBlocks) {
         some.first = b * per_block;
         launch(some, o, (unsigned)(blocks - b < kMostBlocks ? blocks - b : kMostBlocks));
         e = hipGetLastError();
-        if constexpr (OP::kLoss) o.block_loss += kMostBlocks;
+        if constexpr (OP::kLoss)
+            if (o.block_loss) o.block_loss += kMostBlocks;
     }
     return {e, blocks};
 }
@@ -861,7 +861,7 @@ Launched type_logprobs(const Rows &r, const int32_t *moves, float *logprob, floa
 template <typename T>
 Launched type_policy_loss(const Rows &r, const PolicyLoss &p, hipStream_t stream) {
     const PolicyOp op = {p.moves, p.shares, p, p.grad && aligned_with<T>(r, p.grad, p.grad_stride)};
-    return run<T>(r, op, wide_of<T>(r, p.shares, r.rows * 4), stream);
+    return run<T>(r, op, wide_of<T>(r, p.shares, r.rows * 8), stream);
 }
 
 template <typename T>

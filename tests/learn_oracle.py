@@ -7,7 +7,7 @@ d = m - x:
   S            terms that are off by (3 dbar + 2) U on the average, dbar = sum p d, and a tree of sums:
                (3 dbar + 2 + n/64 + 16) U (a lane adds n/64 of them one after another at most, then come the lanes and wavefronts)
   p            the sum of both, and a reciprocal and a product: (3 (d + dbar) + n/64 + 24) U
-  log S        S's, and 2 U from the logarithm of a number between 0.7 and 1.42 (two steps of at most 2^-25)
+  log S        S's, and 2 U for the logarithm (which is taken in 64 bits)
 """
 import numpy as np
 
