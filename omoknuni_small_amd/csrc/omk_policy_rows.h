@@ -735,7 +735,7 @@ static inline int64_t vectors_of(const Rows &r) {
     return (most + V - 1) / V;
 }
 
-// Blocks of a launch, which leave a share of the loss each (rows, where they are cut).
+// Blocks of a launch, which leave a share of the loss each (rows, where they are cut).  A single one writes the loss itself.
 struct Launched {
     hipError_t error;
     int64_t shares;
@@ -816,8 +816,11 @@ static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_
         // blocks of 256, 64 rows 7.5 and 11.2 us, 1024 rows 22.1 and 18.2 us)
         return r.rows <= 512 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
     }
-    k_parts<ONCE, T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, op, w);
-    k_apply<ONCE, T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, op, w);
+    OP o = op;
+    if constexpr (OP::kLoss)
+        if (r.rows == 1) o.block_loss = nullptr;  // its share is the loss
+    k_parts<ONCE, T, OP><<<(unsigned)(r.rows * w.pieces), kPieceBlock, 0, stream>>>(r, o, w);
+    k_apply<ONCE, T, OP><<<(unsigned)(OP::kElements ? r.rows * w.pieces : r.rows), kPieceBlock, 0, stream>>>(r, o, w);
     return {hipGetLastError(), r.rows};
 }
 

@@ -1,0 +1,53 @@
+"""Calls on rows of logits that the tables of the other tests leave out: single rows of every width, rows of which a part holds
+the type's lowest value, references far from the policy, and what lies at the ends of their ranges.  Against 64 bits, with
+tolerances that count what is rounded."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U = 2.0 ** -24  # half a step of a 32-bit float
+
+
+@pytest.fixture(scope="module")
+def learner():
+    import omoknuni_small_amd as omk
+    return omk.Learner()
+
+
+def poison(learner, elements):
+    """Memory of the sizes that the next calls ask for holds what is no result."""
+    held = [torch.full((n,), 12345.0, device="cuda") for n in (elements, 4096, 64, 16) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", [1, 2, 225, 1500, 5000, 40000, 65528, 65529, 65537, 70001, 300000])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_a_single_row_of_any_width(learner, kind, actions, rows):
+    """A row's loss is its share: -ratio * advantage where nothing is clipped.  (One row's share is the whole loss in every kernel;
+    two rows' are added up by another.)"""
+    gen = torch.Generator().manual_seed(actions)
+    x = torch.randn(rows, actions, generator=gen).to(TYPES[kind])
+    moves = torch.randint(0, actions, (rows,), generator=gen, dtype=torch.int32)
+    lp = torch.log_softmax(x.double(), 1).gather(1, moves[:, None].long())[:, 0]
+    old = (lp + 0.05).float()
+    advantage = torch.tensor([1.5, 0.25][:rows])
+    want = -(torch.exp(lp - old.double()) * advantage.double()).sum() * 0.5
+    poison(learner, rows * actions)
+    got = learner.policy_loss(x.cuda(), moves.cuda(), old.cuda(), advantage.cuda(), scale=0.5)
+    # the loss is rounded once; a log-probability is off by what the terms of its sum are: a few roundings each
+    assert abs(float(got.loss) - float(want)) <= 8 * U * abs(float(want)) + U * abs(float(want))
+    p = torch.softmax(x.double(), 1)
+    slope = -(torch.exp(lp - old.double()) * advantage.double()) * 0.5
+    one = torch.zeros_like(p).scatter_(1, moves[:, None].long(), 1.0)
+    half = {"f32": U, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[kind]
+    g = slope[:, None] * (one - p)
+    # 16 roundings of a probability or of the 1 beside it, and the result's own
+    off = slope.abs()[:, None] * (p + one) * 16 * U + g.abs() * half + (2.0 ** -25 if kind == "f16" else 2.0 ** -126)
+    assert ((got.grad.double().cpu() - g).abs() <= off).all()
