@@ -281,6 +281,13 @@ struct LineOp {
 
 // ---- rows that registers hold ----
 
+// sum exp(x - m) (x - m) of terms relative to their own maximum m, relative to one that is -d larger: f is exp(d).  (d is bounded
+// as single terms' differences are below: where f is 0 long since, a sum of terms at the type's lowest value times d would
+// be infinite, and the product no number.)
+__device__ __forceinline__ float moved(float centred, float sum, float d, float f) {
+    return (centred + sum * fmaxf(d, -200.0f)) * f;
+}
+
 // Joins the maxima and sums of a block's wavefronts, whose terms are relative to their own maxima until then: one
 // exchange through LDS serves both.  Every thread of the block calls it; the result is the same in all of them.
 template <bool CENTRED, int WAVES>
@@ -303,7 +310,7 @@ __device__ __forceinline__ RowStats join_waves(float top, double sum, float cent
         const bool empty = tops[w] == -INFINITY;  // (its sum is 0, or NaN)
         const float d = empty ? 0.0f : tops[w] - all.top, f = exp_of<true>(d);
         all.sum += sums[w] * (double)f;
-        if (CENTRED) all.centred += (centreds[w] + (float)sums[w] * d) * f;
+        if (CENTRED) all.centred += moved(centreds[w], (float)sums[w], d, f);
     }
     return all;
 }
@@ -540,7 +547,7 @@ __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int f
         }
         load(from + kTile * BLOCK);
         const float at = most == -INFINITY ? 0.0f : most, d = top - at, f = exp_of<true>(d);
-        if (CENTRED) centred = top == -INFINITY ? 0.0f : (centred + sum * d) * f;
+        if (CENTRED) centred = top == -INFINITY ? 0.0f : moved(centred, sum, d, f);
         sum *= f;
 #pragma unroll
         for (int k = 0; k < kTile; k++) sum += exponentials<true, CENTRED, V>(x[k], at, x[k], centred);
@@ -549,7 +556,7 @@ __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int f
     // the lanes' maxima and sums, then the wavefronts'
     const float most = team_max<64>(top);
     const float d = top == -INFINITY ? 0.0f : top - most, f = exp_of<true>(d);
-    if (CENTRED) centred = team_sum<64>((centred + sum * d) * f);
+    if (CENTRED) centred = team_sum<64>(moved(centred, sum, d, f));
     return join_waves<CENTRED, BLOCK / 64>(most, team_sum<64>((double)(sum * f)), centred);
 }
 
@@ -610,7 +617,7 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
         const bool empty = parts[i].top == -INFINITY;
         const float d = empty ? 0.0f : parts[i].top - top, f = exp_of<true>(d);
         sum += parts[i].sum * (double)f;
-        if (OP::kCentred) centred += (parts[i].centred + (float)parts[i].sum * d) * f;
+        if (OP::kCentred) centred += moved(parts[i].centred, (float)parts[i].sum, d, f);
     }
     if (OP::kCentred) centred = team_sum<64>(centred);
     const RowStats s = join_waves<OP::kCentred, kPieceBlock / 64>(top, team_sum<64>(sum), centred);

@@ -6,6 +6,8 @@ import math
 import numpy as np
 import pytest
 
+from tests import learn_oracle as O
+
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +53,30 @@ def test_a_single_row_of_any_width(learner, kind, actions, rows):
     # 16 roundings of a probability or of the 1 beside it, and the result's own
     off = slope.abs()[:, None] * (p + one) * 16 * U + g.abs() * half + (2.0 ** -25 if kind == "f16" else 2.0 ** -126)
     assert ((got.grad.double().cpu() - g).abs() <= off).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", [225, 1500, 3000, 20011, 50000, 150000])
+@pytest.mark.parametrize("where", ["first half", "last half", "all but one", "all but the last", "every other thousand"])
+def test_columns_of_the_lowest_value(learner, kind, actions, where):
+    """Actions masked by the type's lowest finite value, as they are where no bit masks are used: probability 0, and nothing
+    to the entropy."""
+    rng = np.random.default_rng(actions)
+    dtype = TYPES[kind]
+    x = torch.from_numpy(rng.normal(0, 2, (5, actions))).to(dtype)
+    j = torch.arange(actions)
+    masked = {"first half": j < actions // 2, "last half": j >= actions // 2, "all but one": j != actions // 3,
+              "all but the last": j < actions - 1, "every other thousand": j // 1000 % 2 == 0}[where]
+    if masked.all():
+        masked[7] = False
+    x[1:4, masked] = torch.finfo(dtype).min
+    x[3, :] = torch.finfo(dtype).min
+    o = O.Rows(x.double().numpy())
+    moves = torch.from_numpy(o.p.argmax(1).astype(np.int32))
+    got = learner.logprobs(x.cuda(), moves.cuda(), entropy=True)
+    entropy = got.entropy.double().cpu().numpy()
+    assert (np.abs(entropy - o.entropy) <= o.entropy_off()).all()
+    lp, _, off = o.taken(moves.numpy())
+    assert (np.abs(got.logprob.double().cpu().numpy() - lp) <= off + np.abs(lp) * U).all()
+    p = learner.priors(x.cuda()).double().cpu().numpy()
+    assert (np.abs(p - o.p) <= o.priors_off()).all()
