@@ -124,7 +124,7 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
  * gives it as d_line_logprob (which must not overlap it).  d_line_begin must not decrease.  (Bounds that do not fit
  * are taken as the nearest that do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
  * empty; which line's gradient a row of two lines gets is open.)  Rows before the first line and behind the last are not
- * read.  0 .. OMK_MAX_PAIRS pairs. */
+ * read.  0 .. OMK_MAX_PAIRS pairs; with 0 the loss is 0, and every row is a row of no line (zero_rest). */
 typedef struct omk_preference_params {
     double beta;
     double label_smoothing; /* 0 .. 0.5 */

@@ -299,11 +299,10 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
     if (!out->d_loss) return learn_fail(OMK_ERR_INVALID, "%s: no loss", who);
     const void *all[] = {d_moves, d_line_begin, d_ref_logprob, out->d_loss, out->d_margin, out->d_line_logprob};
     if (!aligned4(who, all, 6)) return OMK_ERR_INVALID;
+    if (r.rows && out->d_grad)
+        if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true)) return rc;
     if (pairs) {
         if (!d_line_begin || (r.rows && !d_moves)) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
-        if (r.rows && out->d_grad)
-            if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
-                return rc;
         const struct {
             const void *to;
             int64_t bytes;
@@ -316,7 +315,7 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);
-    if (!pairs) {
+    if (!pairs && !(r.rows && out->d_grad && out->zero_rest)) {
         LEARN_TRY(launch_set_float(out->d_loss, 0.0f, l->stream));
         return OMK_OK;
     }

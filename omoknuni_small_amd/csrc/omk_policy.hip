@@ -102,13 +102,18 @@ hipError_t launch_policy_loss(int type, const Rows &r, const PolicyLoss &p, hipS
 }
 
 hipError_t launch_preference_loss(int type, const Rows &r, const PreferenceLoss &p, int64_t before, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    if (!p.pairs) {  // rows of no line: the gradient's launch sets them, and the loss, to 0
+        OMK_BY_TYPE(type, e = type_line_gradient<T>(r, p, stream));
+        return e;
+    }
     if (r.rows) {
         Launched l;
         OMK_BY_TYPE(type, l = type_lines<T>(r, p, before, stream));
         if (l.error != hipSuccess) return l.error;
     }
     k_pairs<<<(unsigned)p.pairs, 256, 0, stream>>>(r, p);
-    hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (p.grad) {
         OMK_BY_TYPE(type, e = type_line_gradient<T>(r, p, stream));

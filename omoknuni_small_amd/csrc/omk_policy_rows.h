@@ -247,12 +247,14 @@ struct PolicyOp {
     }
 };
 
-// The rows that lines hold: from line_begin's first to its last, inside the rows there are.
+// The rows that lines hold: from line_begin's first to its last, inside the rows there are.  (None without pairs, where
+// line_begin may be NULL.)
 struct LineRows {
     int64_t begin, end;
     __device__ int64_t inside(int64_t at) const { return at < begin ? begin : at > end ? end : at; }
 };
 __device__ __forceinline__ LineRows line_rows(const PreferenceLoss &p, int64_t rows) {
+    if (p.pairs == 0) return {0, 0};
     const LineRows all = {0, rows};
     const int64_t begin = all.inside(p.line_begin[0]), end = all.inside(p.line_begin[2 * p.pairs]);
     return {begin, end < begin ? begin : end};

@@ -80,3 +80,31 @@ def test_columns_of_the_lowest_value(learner, kind, actions, where):
     assert (np.abs(got.logprob.double().cpu().numpy() - lp) <= off + np.abs(lp) * U).all()
     p = learner.priors(x.cuda()).double().cpu().numpy()
     assert (np.abs(p - o.p) <= o.priors_off()).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,actions", [(1, 1), (37, 225), (70, 362), (9, 5000), (3, 70001)])
+def test_rows_without_a_pair(learner, kind, rows, actions):
+    """No line of play: the loss is 0, a new gradient is 0 everywhere, and a given one is left as it is."""
+    x = torch.randn(rows, actions, device="cuda").to(TYPES[kind])
+    moves = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    begin = torch.full((1,), 7, dtype=torch.int32, device="cuda")
+    poison(learner, rows * actions)
+    poison(learner, (rows * actions + 1) // 2)
+    got = learner.preference_loss(x, moves, begin)
+    assert float(got.loss) == 0 and got.grad.shape == x.shape and (got.grad == 0).all()
+    assert got.margin.shape == (0,) and got.logprob.shape == (0,)
+    assert float(learner.preference_loss(x, moves, begin, grad=False).loss) == 0
+    given = torch.full_like(x, 7.0)
+    assert float(learner.preference_loss(x, moves, begin, grad=given).loss) == 0 and (given == 7).all()
+    # rows with gaps, through the C ABI: what lies between two rows stays
+    from omoknuni_small_amd import learn
+    import ctypes as C
+    wide = torch.full((rows, actions + 3), 7.0, dtype=TYPES[kind], device="cuda")
+    loss = torch.full((), 7.0, device="cuda")
+    r = learn._Rows(x.data_ptr(), actions, rows, actions, learner._types[x.dtype], None, 0)
+    out = learn._PreferenceOut(loss.data_ptr(), wide.data_ptr(), actions + 3, None, None, 1)
+    learner._on_stream()
+    rc = learn._library().omk_preference_loss(learner._h, C.byref(r), None, None, 0, None, C.byref(learn._PreferenceParams(0.1, 0.0, 1.0)),
+                                              C.byref(out), None, 0)
+    assert rc == 0 and float(loss) == 0 and (wide[:, :actions] == 0).all() and (wide[:, actions:] == 7).all()
