@@ -108,3 +108,40 @@ def test_rows_without_a_pair(learner, kind, rows, actions):
     rc = learn._library().omk_preference_loss(learner._h, C.byref(r), None, None, 0, None, C.byref(learn._PreferenceParams(0.1, 0.0, 1.0)),
                                               C.byref(out), None, 0)
     assert rc == 0 and float(loss) == 0 and (wide[:, :actions] == 0).all() and (wide[:, actions:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("actions", [2, 225, 3000, 40000, 70001])
+def test_references_near_and_far(learner, kind, actions):
+    """The KL term alone (no advantage): kl = exp(d) - d - 1 and the slope exp(d) - 1 for references from where the policy is to
+    ones that never play the move, and ones that nearly always do."""
+    ds = np.array([0, 1e-4, -1e-4, 1e-3, -1e-3, 0.01, -0.01, 0.015, 0.017, -0.24, 0.24, -0.26, 0.26, 1, -1, -3, -10, -1e3, -1e5, -1e9, -3e38, -np.inf, 5, 20])
+    rng = np.random.default_rng(actions)
+    x = torch.from_numpy(rng.normal(0, 1, (len(ds), actions))).to(TYPES[kind])
+    o = O.Rows(x.double().numpy())
+    moves = rng.integers(0, actions, len(ds)).astype(np.int32)
+    lp, _, off = o.taken(moves)
+    ref = (lp + ds).astype(np.float32)
+    d = ref.astype(np.float64) - lp
+    zero = torch.zeros(len(ds), device="cuda")
+    got = learner.policy_loss(x.cuda(), torch.from_numpy(moves).cuda(), torch.from_numpy(lp.astype(np.float32)).cuda(), zero,
+                              ref_logprob=torch.from_numpy(ref).cuda(), kl_weight=0.5, scale=2.0)
+    slope, kl = -np.expm1(d), np.expm1(d) - d
+    kl[np.abs(d) < 1e-5] = (d * d / 2)[np.abs(d) < 1e-5]
+    # both are worked out in 64 bits from a log-probability that is `off` off, and rounded once (the slope, a probability and their
+    # product: three times)
+    kl_off = np.abs(slope) * off + np.exp(d) * off ** 2 + kl * U * 1.01
+    mine = got.kl.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        assert ((np.abs(mine - kl) <= kl_off) | (mine == kl)).all()
+    assert np.isinf(mine[21]) and float(got.loss) == np.inf
+    g, g_off = o.gradient(moves, slope, np.exp(d) * off + np.abs(slope) * 4 * U, kind)
+    mine = got.grad.double().cpu().numpy()
+    assert (np.abs(mine - g) <= g_off).all()
+    # without the infinite one the loss is the divergences' sum
+    keep = [i for i in range(len(ds)) if i != 21]
+    put = lambda a: torch.from_numpy(a[keep]).cuda()  # noqa: E731
+    got = learner.policy_loss(x[keep].cuda(), put(moves), put(lp.astype(np.float32)), zero[:len(keep)], ref_logprob=put(ref), kl_weight=1e-30,
+                              scale=2.0)
+    want = 2e-30 * kl[keep].sum()
+    assert abs(float(got.loss) - want) <= 2 * U * want
