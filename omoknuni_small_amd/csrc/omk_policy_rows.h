@@ -103,18 +103,6 @@ __device__ __forceinline__ void store_vector(OUT *out, bool aligned, int j, int 
         if (j + i >= 0 && j + i < actions) out[j + i] = (OUT)y[i];
 }
 
-template <int V>
-__device__ __forceinline__ float sum_of(const float (&e)[V]) {
-    float s[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) s[i] = e[i];
-#pragma unroll
-    for (int d = V / 2; d; d >>= 1)
-#pragma unroll
-        for (int i = 0; i < d; i++) s[i] += s[i + d];
-    return s[0];
-}
-
 // ---- what operators do with a row ----
 
 // The move of a row (-1 where it lies outside the action space) and its logit, -inf where it is not legal.
@@ -291,43 +279,51 @@ __device__ __forceinline__ float moved(float centred, float sum, float d, float 
 }
 
 // Joins the maxima and sums of a block's wavefronts, whose terms are relative to their own maxima until then: one
-// exchange through LDS serves both.  Every thread of the block calls it; the result is the same in all of them.
+// exchange through LDS serves both.  Every thread of the block calls it; the result is the same in all of them.  A lane for
+// every wavefront, so that its factor can be taken in 64 bits: in 32 its rounding would be in all of the wavefront's terms alike.
 template <bool CENTRED, int WAVES>
 __device__ __forceinline__ RowStats join_waves(float top, double sum, float centred) {
     __shared__ float tops[WAVES], centreds[WAVES];
     __shared__ double sums[WAVES];
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, of = threadIdx.x & (WAVES - 1);
     if ((threadIdx.x & 63) == 0) {
         tops[wave] = top;
         sums[wave] = sum;
         if (CENTRED) centreds[wave] = centred;
     }
     __syncthreads();
-    RowStats all = {-INFINITY, 0.0f, 0.0};
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) all.top = fmaxf(all.top, tops[w]);
+    const float its = tops[of];
+    RowStats all = {team_max<WAVES>(its), 0.0f, 0.0};
     if (all.top == -INFINITY) all.top = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        const bool empty = tops[w] == -INFINITY;  // (its sum is 0, or NaN)
-        const float d = empty ? 0.0f : tops[w] - all.top, f = exp_of<true>(d);
-        all.sum += sums[w] * (double)f;
-        if (CENTRED) all.centred += moved(centreds[w], (float)sums[w], d, f);
-    }
+    const double d = its == -INFINITY ? 0.0 : (double)its - (double)all.top, f = exp(d);  // (an empty one's sum is 0, or NaN)
+    all.sum = team_sum<WAVES>(sums[of] * f);
+    if (CENTRED) all.centred = team_sum<WAVES>(moved(centreds[of], (float)sums[of], (float)d, (float)f));
     return all;
 }
 
-// exp(x - m) of a vector's elements and their sum; with CENTRED also adds exp(x - m) (x - m) up, where a term whose exponential
-// is 0 (x = -inf among them) counts nothing and one that is no number shows.
+// exp(x - m) of a vector's elements; with CENTRED also adds exp(x - m) (x - m) up, where a term whose exponential is 0 (x = -inf
+// among them) counts nothing and one that is no number shows.
 template <bool FINE, bool CENTRED, int V>
-__device__ __forceinline__ float exponentials(const float (&x)[V], float top, float (&e)[V], float &centred) {
+__device__ __forceinline__ void exponentials(const float (&x)[V], float top, float (&e)[V], float &centred) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float d = x[i] - top;
+        const float d = FINE ? at_least(x[i] - top, -200.0f) : x[i] - top;
         e[i] = exp_of<FINE>(d);
-        if (CENTRED) centred = __builtin_fmaf(e[i], fmaxf(d, -200.0f), centred);
+        if (CENTRED) centred = __builtin_fmaf(e[i], d, centred);
     }
-    return sum_of<V>(e);
+}
+
+// Their sum.  In 64 bits from the terms on: beside the largest, which is 1, the others of a row that is all but decided would lose
+// their digits, and with them the logarithm of the sum.
+template <int V>
+__device__ __forceinline__ double sum_of(const float (&e)[V]) {
+    double even = (double)e[0], odd = (double)e[1];
+#pragma unroll
+    for (int i = 2; i < V; i += 2) {
+        even += (double)e[i];
+        odd += (double)e[i + 1];
+    }
+    return even + odd;
 }
 
 // The elements of a vector as floats, -inf where they are not the row's or not legal.  LOOK: nearly all vectors of a row
@@ -400,11 +396,15 @@ __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
     }
     top = team_max<TEAM>(top);
     if (top == -INFINITY) top = 0.0f;
-    float sum = 0.0f, centred = 0.0f;
+    double sum = 0.0;
+    float centred = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; k++) sum += exponentials<true, OP::kCentred, V>(e[k], top, e[k], centred);
+    for (int k = 0; k < K; k++) {
+        exponentials<true, OP::kCentred, V>(e[k], top, e[k], centred);
+        sum += sum_of<V>(e[k]);
+    }
     if (OP::kCentred) centred = team_sum<TEAM>(centred);
-    const RowStats s = {top, centred, team_sum<TEAM>((double)sum)};
+    const RowStats s = {top, centred, team_sum<TEAM>(sum)};
     RowOut out = {0.0f, 0.0f, -1, true, 0.0f};
     if (here && sub == 0) out = op.row(row, s, m, true);
 
@@ -476,16 +476,18 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
     }
     top = team_max<64>(top);
     const float own_top = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, centred = 0.0f;
+    double sum = 0.0;
+    float centred = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; k++) {
         float(&x)[V] = e[KEEP ? k : 0];
         if (!KEEP) floats_of<false, T>(p[k], bits[k], x);
-        sum += exponentials<!OP::kElements, OP::kCentred, V>(x, own_top, x, centred);
+        exponentials<true, OP::kCentred, V>(x, own_top, x, centred);
+        sum += sum_of<V>(x);
     }
     if (OP::kCentred) centred = team_sum<64>(centred);
     __shared__ RowOut shared_out;
-    const RowStats s = join_waves<OP::kCentred, WAVES>(top, team_sum<64>((double)sum), centred);
+    const RowStats s = join_waves<OP::kCentred, WAVES>(top, team_sum<64>(sum), centred);
     if (threadIdx.x < 64) {
         const RowOut o = op.row(row, s, m, threadIdx.x == 0);
         if (threadIdx.x == 0) shared_out = o;
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(R
         typedef typename OP::template Element<T> OUT;
         const RowOut out = shared_out;
         if (OUT *to = op.template elements<OUT>(row)) {
-            const float each = out.each * (top == -INFINITY ? 0.0f : exp_of<true>(top - s.top));
+            const float each = out.each * (top == -INFINITY ? 0.0f : exp_of<true>(at_least(top - s.top, -200.0f)));
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int vec = k * TEAM + (int)threadIdx.x;
@@ -521,7 +523,7 @@ constexpr int kTile = 2;  // vectors of a thread at a time
 // A block goes through vectors first .. end - 1 of a row tile by tile with a running maximum and sum: m' = max(m, tile's
 // maximum), s' = s exp(m - m') + sum exp(x - m').  The next tile is on its way while one is looked at, and few registers hold
 // it all, so that eight blocks share a compute unit.  (Tiles of four vectors were slower by a tenth: five blocks.)  2049 rows of 50001
-// f16 with their entropies: 51 us, 4.0 TB/s.
+// f16 with their entropies: 56 us, 3.7 TB/s, bound by instructions: 15 a term, four of them the exponential's.
 template <bool ONCE, typename T, int BLOCK, bool CENTRED>
 __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int first, int end) {
     constexpr int V = Pack<T>::V;
@@ -529,37 +531,56 @@ __device__ __forceinline__ RowStats stream_row(const Rows &r, int64_t row, int f
     const uint32_t *legal = r.legal ? r.legal + row * r.legal_stride : nullptr;
     Pack<T> next[kTile];
     const auto bits_at = [&](int vec) { return vec < end ? inside_bits<V>(vec * V - head, r.actions) : 0u; };
-    const auto load = [&](int from) {
+    // Tiles that lie inside the row are loaded without a look at bounds, and without a mask need none at bits either (the rows
+    // above: 64 us where every tile looks, 56 us so).
+    const T *const at_row = (const T *)r.x + (row * r.stride - head);
+    const int inner_end = min(end, (r.actions + head) / V);
+    const auto inner = [&](int start) { return r.aligned && (start || !head) && start + kTile * BLOCK <= inner_end; };
+    const auto load = [&](int start) {
+        const int from = start + (int)threadIdx.x;
+        if (inner(start)) {
+#pragma unroll
+            for (int k = 0; k < kTile; k++) next[k].raw = load16<ONCE>(at_row + (from + k * BLOCK) * V);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < kTile; k++)
             load_vector<ONCE, T>(r, row, (from + k * BLOCK) * V - head, bits_at(from + k * BLOCK), next[k]);
     };
-    load(first + (int)threadIdx.x);
-    float top = -INFINITY, sum = 0.0f, centred = 0.0f;
+    load(first);
+    float top = -INFINITY, centred = 0.0f;
+    double sum = 0.0;
     for (int start = first; start < end; start += kTile * BLOCK) {
         const int from = start + (int)threadIdx.x;
         float x[kTile][V], most = top;
+        const bool all = !legal && inner(start);
 #pragma unroll
         for (int k = 0; k < kTile; k++) {
-            uint32_t bits = bits_at(from + k * BLOCK);
-            if (legal && bits) bits &= legal_bits(legal, r.words, (from + k * BLOCK) * V - head);
+            uint32_t bits = (1u << V) - 1u;
+            if (!all) {
+                bits = bits_at(from + k * BLOCK);
+                if (legal && bits) bits &= legal_bits(legal, r.words, (from + k * BLOCK) * V - head);
+            }
             floats_of<true, T>(next[k], bits, x[k]);
 #pragma unroll
             for (int i = 0; i < V; i++) most = fmaxf(most, x[k][i]);
         }
-        load(from + kTile * BLOCK);
-        const float at = most == -INFINITY ? 0.0f : most, d = top - at, f = exp_of<true>(d);
-        if (CENTRED) centred = top == -INFINITY ? 0.0f : moved(centred, sum, d, f);
-        sum *= f;
+        load(start + kTile * BLOCK);
+        const float at = most == -INFINITY ? 0.0f : most, d = at_least(top - at, -200.0f), f = exp_of<true>(d);
+        if (CENTRED) centred = top == -INFINITY ? 0.0f : moved(centred, (float)sum, d, f);
+        sum *= (double)f;
 #pragma unroll
-        for (int k = 0; k < kTile; k++) sum += exponentials<true, CENTRED, V>(x[k], at, x[k], centred);
+        for (int k = 0; k < kTile; k++) {
+            exponentials<true, CENTRED, V>(x[k], at, x[k], centred);
+            sum += sum_of<V>(x[k]);
+        }
         top = most;
     }
     // the lanes' maxima and sums, then the wavefronts'
     const float most = team_max<64>(top);
-    const float d = top == -INFINITY ? 0.0f : top - most, f = exp_of<true>(d);
-    if (CENTRED) centred = team_sum<64>(moved(centred, sum, d, f));
-    return join_waves<CENTRED, BLOCK / 64>(most, team_sum<64>((double)(sum * f)), centred);
+    const double d = top == -INFINITY ? 0.0 : (double)top - (double)most, f = exp(d);
+    if (CENTRED) centred = team_sum<64>(moved(centred, (float)sum, (float)d, (float)f));
+    return join_waves<CENTRED, BLOCK / 64>(most, team_sum<64>(sum * f), centred);
 }
 
 template <bool ONCE, typename T, int BLOCK, typename OP>
@@ -617,9 +638,9 @@ __global__ __launch_bounds__(kPieceBlock) void k_apply(Rows r, OP op, Wide w) {
     float centred = 0.0f;
     for (int i = threadIdx.x; i < w.pieces; i += kPieceBlock) {
         const bool empty = parts[i].top == -INFINITY;
-        const float d = empty ? 0.0f : parts[i].top - top, f = exp_of<true>(d);
-        sum += parts[i].sum * (double)f;
-        if (OP::kCentred) centred += moved(parts[i].centred, (float)parts[i].sum, d, f);
+        const double d = empty ? 0.0 : (double)parts[i].top - (double)top, f = exp(d);
+        sum += parts[i].sum * f;
+        if (OP::kCentred) centred += moved(parts[i].centred, (float)parts[i].sum, (float)d, (float)f);
     }
     if (OP::kCentred) centred = team_sum<64>(centred);
     const RowStats s = join_waves<OP::kCentred, kPieceBlock / 64>(top, team_sum<64>(sum), centred);

@@ -145,3 +145,60 @@ def test_references_near_and_far(learner, kind, actions):
                               scale=2.0)
     want = 2e-30 * kl[keep].sum()
     assert abs(float(got.loss) - want) <= 2 * U * want
+
+
+WIDTHS = [2, 31, 225, 362, 1500, 5000, 20011, 40000, 70001]  # of every kernel that holds, streams or cuts rows
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", WIDTHS)
+def test_log_probabilities_are_as_exact_as_their_terms(learner, kind, actions):
+    """How far log-probabilities are off before they are rounded, seen through the divergence from a reference close by:
+    kl(d + t) = kl(d) + (exp(d) - 1) t + ..
+
+    Logits are multiples of 1/16, so that differences are exact.  A term exp(x - m) is then off by 4e-8 (rms) and 5e-9 on the mean (two
+    roundings of the instruction and of the correction); sums are exact beside that.  So t has a mean of 5e-9 and a spread of
+    4e-8 sqrt(sum p^2); six of these are allowed, and the divergence's own rounding, U d/2."""
+    rng = np.random.default_rng(actions)
+    rows = max(8, min(400, 2000000 // actions))
+    x = np.round(rng.normal(0, 2, (rows, actions)).clip(-7, 7) * 16) / 16
+    if actions > 1000:
+        x[0] = -3.0
+        x[0, actions // 2:] = 2.5  # the largest logits all in one half: the other's sums are relative to another maximum
+    o = O.Rows(x)
+    moves = rng.integers(0, actions, rows).astype(np.int32)
+    lp, _, _ = o.taken(moves)
+    ref = (lp + 0.01).astype(np.float32)
+    d = ref.astype(np.float64) - lp
+    zero = torch.zeros(rows, device="cuda")
+    got = learner.policy_loss(torch.from_numpy(x).to(TYPES[kind]).cuda(), torch.from_numpy(moves).cuda(), zero, zero,
+                              ref_logprob=torch.from_numpy(ref).cuda())
+    kl = np.expm1(d) - d
+    off = 5e-9 + 6 * 4e-8 * np.sqrt((o.p ** 2).sum(1)) * (o.p.max(1) < 1)
+    t = (got.kl.double().cpu().numpy() - kl) / np.expm1(d)
+    assert (np.abs(t) <= off + U * np.abs(d)).all(), np.abs(t / off).max()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", WIDTHS)
+def test_rows_that_are_all_but_decided(learner, kind, actions):
+    """One action far above the others: log-probability -log(1 + (n - 1) exp(-gap)) and entropy keep their digits beside the 1.
+
+    Every other term is off by a step of the exponential (2 U) and the correction's rounding (U), the sum of them by nothing, and
+    the result is rounded (U)."""
+    gaps = np.array([3.0, 8.0, 11.0, 13.0, 15.0, 17.0])
+    x = np.zeros((len(gaps), actions))
+    at = np.arange(len(gaps)) * (actions - 1) // (len(gaps) - 1)
+    x[np.arange(len(gaps)), at] = gaps
+    rest = (actions - 1) * np.exp(-gaps)
+    got = learner.logprobs(torch.from_numpy(x).to(TYPES[kind]).cuda(), torch.from_numpy(at.astype(np.int32)).cuda(), entropy=True)
+    lp = -np.log1p(rest)
+    assert (np.abs(got.logprob.double().cpu().numpy() - lp) <= 4.1 * U * np.abs(lp)).all()
+    entropy = np.log1p(rest) + rest * gaps / (1 + rest)
+    # the second part adds terms of one size up in 32 bits: n/64 of them one after another at most, then lanes and wavefronts
+    off = 4.1 * U * np.log1p(rest) + (actions / 64 + 24) * U * rest * gaps / (1 + rest) + 2 * U * entropy
+    assert (np.abs(got.entropy.double().cpu().numpy() - entropy) <= off).all()
+    lines = learner.preference_loss(torch.from_numpy(x).to(TYPES[kind]).cuda(), torch.from_numpy(at.astype(np.int32)).cuda(),
+                                    torch.tensor([0, 1, 6], dtype=torch.int32, device="cuda"), grad=False).logprob.double().cpu().numpy()
+    want = np.array([lp[0], lp[1:].sum()])
+    assert (np.abs(lines - want) <= 4.1 * U * np.abs(want)).all()
