@@ -119,8 +119,8 @@ __device__ __forceinline__ Move move_of(const Rows &r, const int32_t *moves, int
     return m;
 }
 
-// The result of an operator's look at a row: element j becomes each * exp(x_j - top), and at_move more where j is the
-// move; 0 wherever `none`.
+// The result of an operator's look at a row: element j becomes each * exp(x_j - top), and at_move where j is the move (a
+// gradient's slope * (1 - p), by itself: as slope and slope * -p it would lose its digits where p is nearly 1); 0 wherever `none`.
 struct RowOut {
     float each, at_move;
     int32_t move;
@@ -201,11 +201,12 @@ struct PolicyOp {
     }
     __device__ RowOut row(int64_t row, const RowStats &s, Move m, bool writes) const {
         // (in 64 bits up to the sum: advantages have a mean of about 0, and what is left of a sum of rows is small beside them)
-        double loss = 0.0, slope = 0.0;
+        double loss = 0.0, slope = 0.0, others = 0.0;  // (probability of the other actions)
         float lp = 0.0f, kl = 0.0f;
         if (m.chosen != -INFINITY) {
             const double exact = (double)m.chosen - (double)s.top - log(s.sum);
             lp = (float)exact;
+            if (p.grad) others = 1.0 - exp(exact);
             const float a = p.advantage[row];
             const double shift = exact - (double)p.old_logprob[row];
             if (a > 0.0f ? shift > p.log_high : a < 0.0f && shift < p.log_low) {
@@ -230,8 +231,8 @@ struct PolicyOp {
             if (p.kl) p.kl[row] = kl;
         }
         const float by_logprob = (float)slope;
-        return {by_logprob == 0.0f ? 0.0f : -by_logprob * __builtin_amdgcn_rcpf((float)s.sum), by_logprob, m.move,
-                by_logprob == 0.0f, loss};
+        return {by_logprob == 0.0f ? 0.0f : -by_logprob * __builtin_amdgcn_rcpf((float)s.sum),
+                by_logprob == 0.0f ? 0.0f : (float)(slope * others), m.move, by_logprob == 0.0f, loss};
     }
 };
 
@@ -345,7 +346,7 @@ __device__ __forceinline__ void floats_of(const Pack<T> &p, uint32_t bits, float
     }
 }
 
-// Writes a vector of a row's results: exp(x - m) times `each`, and `at_move` more at element `at` (counted from the first
+// Writes a vector of a row's results: exp(x - m) times `each`, but `at_move` at element `at` (counted from the first
 // vector's first; -1: nowhere), or 0.
 template <bool ONCE, typename T, typename OUT>
 __device__ __forceinline__ void write_vector(OUT *to, bool aligned, int vec, int head, int actions, const float (&e)[Pack<T>::V],
@@ -356,7 +357,7 @@ __device__ __forceinline__ void write_vector(OUT *to, bool aligned, int vec, int
     for (int i = 0; i < V; i++) y[i] = none ? 0.0f : e[i] * each;
     if (at >= 0 && at / V == vec) {
 #pragma unroll
-        for (int i = 0; i < V; i++) y[i] += at % V == i ? at_move : 0.0f;
+        for (int i = 0; i < V; i++) y[i] = at % V == i ? at_move : y[i];
     }
     store_vector<ONCE, T, OUT>(to, aligned, vec * V - head, actions, y);
 }
@@ -728,8 +729,10 @@ __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p,
     if (rest && !p.zero_rest) return;
     const float slope = rest ? 0.0f : p.slope[row], top = rest ? 0.0f : p.top[row];
     const float each = rest ? 0.0f : -slope * p.inverse[row];
-    const int head = head_of<T>(r, row), first = (int)(item % pieces) * (K * 64) + lane;
+    const int piece = (int)(item % pieces), head = head_of<T>(r, row), first = piece * (K * 64) + lane;
     const int at = slope == 0.0f ? -1 : p.moves[row] + head;
+    float at_move = 0.0f;
+    if (at >= 0 && at / (V * K * 64) == piece) at_move = (float)((double)slope * (1.0 - exp(p.logprob[row])));
     T *to = (T *)p.grad + row * p.grad_stride;
     Pack<T> x[K];
     uint32_t bits[K];
@@ -751,7 +754,7 @@ __global__ __launch_bounds__(256) void k_line_gradient(Rows r, PreferenceLoss p,
         float e[V], unused = 0.0f;
         floats_of<true, T>(x[k], bits[k], e);
         exponentials<false, false, V>(e, top, e, unused);
-        write_vector<ONCE, T, T>(to, aligned, vec, head, r.actions, e, each, slope == 0.0f, at, slope);
+        write_vector<ONCE, T, T>(to, aligned, vec, head, r.actions, e, each, slope == 0.0f, at, at_move);
     }
 }
 

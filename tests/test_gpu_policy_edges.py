@@ -202,3 +202,40 @@ def test_rows_that_are_all_but_decided(learner, kind, actions):
                                     torch.tensor([0, 1, 6], dtype=torch.int32, device="cuda"), grad=False).logprob.double().cpu().numpy()
     want = np.array([lp[0], lp[1:].sum()])
     assert (np.abs(lines - want) <= 4.1 * U * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", WIDTHS)
+@pytest.mark.parametrize("which", ["policy", "lines"])
+def test_gradients_of_rows_that_are_all_but_decided(learner, kind, actions, which):
+    """The gradient at a move that is nearly certain is slope * (1 - p): as exact as the others, to which it adds up to 0.
+
+    1 - p is good to two steps of the exponential and a rounding (3 U) and the product is rounded, the slope before it; the other
+    actions' probabilities are off by 3 U, the sum's rounding, a reciprocal to a step (2 U) and three products."""
+    gaps = np.array([3.0, 8.0, 11.0, 13.0, 15.0, 17.0])
+    x = np.zeros((len(gaps), actions))
+    at = np.arange(len(gaps)) * (actions - 1) // (len(gaps) - 1)
+    x[np.arange(len(gaps)), at] = gaps
+    e = np.exp(-gaps)
+    rest = (actions - 1) * e
+    dx, moves = torch.from_numpy(x).to(TYPES[kind]).cuda(), torch.from_numpy(at.astype(np.int32)).cuda()
+    scale = 4096.0  # (in 16 bits with a narrow range these would be next to its end)
+    lp = -np.log1p(rest)
+    if which == "policy":
+        got = learner.policy_loss(dx, moves, torch.from_numpy(lp.astype(np.float32)).cuda(), torch.ones(len(gaps), device="cuda"), scale=scale)
+        slope = -scale * np.exp(lp - lp.astype(np.float32))
+    else:
+        got = learner.preference_loss(dx, moves, torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda"), beta=0.5, scale=scale)
+        u = 0.5 * (lp[:2].sum() - lp[2:].sum())
+        slope = -0.5 * scale / (1 + np.exp(u)) * np.where(np.arange(6) < 2, 1, -1)
+    grad = got.grad.double().cpu().numpy()
+    half, tiny = {"f32": (U, 2.0 ** -126), "bf16": (2.0 ** -8, 2.0 ** -126), "f16": (2.0 ** -11, 2.0 ** -25)}[kind]
+    # (the pairs' slope is worked out in 32 bits: expf, a sum, a quotient, two products)
+    slope_rel = U if which == "policy" else 16 * U
+    want = slope * rest / (1 + rest)
+    assert (np.abs(grad[np.arange(6), at] - want) <= np.abs(want) * (4.1 * U + slope_rel + half) + tiny).all()
+    grad[np.arange(6), at] = np.nan
+    want = np.where(np.isnan(grad), np.nan, (-slope * e / (1 + rest))[:, None])
+    # (by the form without the correction where terms are computed again: x U and 2.2e-8 x more)
+    off = np.abs(want) * (10 * U + 2 * gaps[:, None] * U + slope_rel + half) + tiny
+    assert ((np.abs(grad - want) <= off) | np.isnan(want)).all()
