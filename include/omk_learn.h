@@ -87,7 +87,8 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
  *   l     = -min(ratio * advantage, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantage)
  *           + kl_weight * kl,   kl = exp(ref_logprob - lp) - (ref_logprob - lp) - 1
  *   loss  = scale * sum over rows of weight * l
- * and the gradient of the loss by every logit.  An advantage of 0 gives no loss at whatever ratio, and a row of weight 0
+ * and the gradient of the loss by every logit.  (A derivative by lp that passes the 32-bit range is held at its end, so that an
+ * illegal action's gradient is 0 beside it too; the loss is infinite there.)  An advantage of 0 gives no loss at whatever ratio, and a row of weight 0
  * adds nothing to loss and gradient, whatever its other columns hold.  Results of a row each (d_logprob, d_kl) must not
  * overlap what is read. */
 typedef struct omk_policy_samples {

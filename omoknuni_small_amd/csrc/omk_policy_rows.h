@@ -180,6 +180,13 @@ __device__ __forceinline__ Divergence divergence(double d) {
     return {value, d + value};
 }
 
+// A derivative by a log-probability, as a 32-bit number: held at the ends of their range, since times the probability 0 of an
+// illegal action an infinite one would be no number.  (NaN stays.)
+__device__ __forceinline__ double in_range(double slope) {
+    const double most = 0x1.fffffep127;
+    return slope > most ? most : slope < -most ? -most : slope;
+}
+
 struct PolicyOp {
     static constexpr bool kCentred = false, kElements = true, kMoves = true, kLoss = true;
     template <typename T>
@@ -230,6 +237,7 @@ struct PolicyOp {
             p.logprob[row] = lp;
             if (p.kl) p.kl[row] = kl;
         }
+        slope = in_range(slope);
         const float by_logprob = (float)slope;
         return {by_logprob == 0.0f ? 0.0f : -by_logprob * __builtin_amdgcn_rcpf((float)s.sum),
                 by_logprob == 0.0f ? 0.0f : (float)(slope * others), m.move, by_logprob == 0.0f, loss};

@@ -239,3 +239,21 @@ def test_gradients_of_rows_that_are_all_but_decided(learner, kind, actions, whic
     # (by the form without the correction where terms are computed again: x U and 2.2e-8 x more)
     off = np.abs(want) * (10 * U + 2 * gaps[:, None] * U + slope_rel + half) + tiny
     assert ((np.abs(grad - want) <= off) | np.isnan(want)).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("actions", [225, 3000, 40000, 70001])
+def test_ratios_beyond_the_range(learner, kind, actions):
+    """A ratio that no 32-bit number holds: illegal actions' gradients are 0 all the same, and nothing is NaN."""
+    import omoknuni_small_amd as omk
+    gen = torch.Generator().manual_seed(actions)
+    mask = torch.rand(4, actions, generator=gen) < 0.5
+    mask[:, 3] = True
+    x = torch.randn(4, actions, generator=gen).to(TYPES[kind]).masked_fill(~mask, float("nan")).cuda()
+    moves = torch.full((4,), 3, dtype=torch.int32, device="cuda")
+    old = torch.tensor([-300.0, -math.inf, -3.0, -300.0], device="cuda")
+    adv = torch.tensor([-1.0, -1.0, -1.0, 1.0], device="cuda")  # (the last is clipped)
+    got = learner.policy_loss(x, moves, old, adv, legal=omk.pack_legal(mask).cuda(), scale=1.0)
+    assert float(got.loss) == math.inf
+    assert not got.grad.isnan().any() and (got.grad[~mask.cuda()] == 0).all() and (got.grad[3] == 0).all()
+    assert (got.grad[:2, 3].float() >= (60000 if kind == "f16" else 1e38)).all()
