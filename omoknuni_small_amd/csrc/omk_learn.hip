@@ -324,9 +324,9 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
     p.line_begin = d_line_begin;
     p.pairs = pairs;
     p.ref_logprob = d_ref_logprob;
-    p.beta = (float)params->beta;
-    p.smoothing = (float)params->label_smoothing;
-    p.scale = (float)params->scale;
+    p.beta = params->beta;
+    p.smoothing = params->label_smoothing;
+    p.scale = params->scale;
     p.grad = r.rows ? out->d_grad : nullptr;
     p.grad_stride = out->grad_stride;
     p.zero_rest = out->zero_rest;

@@ -46,7 +46,7 @@ struct PreferenceLoss {
     const int32_t *moves, *line_begin;
     int64_t pairs;
     const float *ref_logprob;
-    float beta, smoothing, scale;
+    double beta, smoothing, scale;
     void *grad;
     int64_t grad_stride;
     int32_t zero_rest;

@@ -33,17 +33,18 @@ __global__ __launch_bounds__(256) void k_pairs(Rows r, PreferenceLoss p) {
         sums[0] -= (double)p.ref_logprob[2 * pair];
         sums[1] -= (double)p.ref_logprob[2 * pair + 1];
     }
-    const float u = (float)((double)p.beta * (sums[0] - sums[1]));
+    // (in 64 bits: where a pair's loss is least, with smoothing, its slope is what is left of two terms)
+    const double u = p.beta * (sums[0] - sums[1]);
     // log(1 + exp(-|u|)), of which both losses are made
-    const float t = expf(-fabsf(u)), rest = log1pf(t);
-    float loss = (1.0f - p.smoothing) * (fmaxf(-u, 0.0f) + rest);
-    if (p.smoothing > 0.0f) loss += p.smoothing * (fmaxf(u, 0.0f) + rest);  // (an infinite margin is no NaN)
-    const float lesser = t / (1.0f + t), greater = 1.0f / (1.0f + t);  // sigmoid(-|u|), sigmoid(|u|)
-    const float above = u >= 0.0f ? greater : lesser, below = u >= 0.0f ? lesser : greater;  // sigmoid(u), sigmoid(-u)
-    const float slope = -p.beta * p.scale * ((1.0f - p.smoothing) * below - p.smoothing * above);
+    const double t = exp(-fabs(u)), rest = log1p(t);
+    double loss = (1.0 - p.smoothing) * (fmax(-u, 0.0) + rest);
+    if (p.smoothing > 0.0) loss += p.smoothing * (fmax(u, 0.0) + rest);  // (an infinite margin is no NaN)
+    const double lesser = t / (1.0 + t), greater = 1.0 / (1.0 + t);  // sigmoid(-|u|), sigmoid(|u|)
+    const double above = u >= 0.0 ? greater : lesser, below = u >= 0.0 ? lesser : greater;  // sigmoid(u), sigmoid(-u)
+    const float slope = (float)in_range(-p.beta * p.scale * ((1.0 - p.smoothing) * below - p.smoothing * above));
     if (threadIdx.x == 0) {
-        if (p.margin) p.margin[pair] = u;
-        p.pair_loss[pair] = p.scale * loss;
+        if (p.margin) p.margin[pair] = (float)u;
+        p.pair_loss[pair] = (float)(p.scale * loss);
     }
     if (!p.grad) return;
     for (int64_t row = begin + half; row < end; row += 128)

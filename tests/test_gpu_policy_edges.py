@@ -257,3 +257,30 @@ def test_ratios_beyond_the_range(learner, kind, actions):
     assert float(got.loss) == math.inf
     assert not got.grad.isnan().any() and (got.grad[~mask.cuda()] == 0).all() and (got.grad[3] == 0).all()
     assert (got.grad[:2, 3].float() >= (60000 if kind == "f16" else 1e38)).all()
+
+
+@pytest.mark.parametrize("beta,smoothing", [(0.5, 0.1), (0.3, 0.25), (0.1, 0.0), (0.7, 0.5)])
+def test_slopes_of_pairs_next_to_their_least_loss(learner, beta, smoothing):
+    """Two actions alike, so that log-probabilities are -log 2 exactly (to 2^-53): the margin is what the references make it, and
+    the gradient slope / 2.  Each result is rounded to 32 bits once; the gradient's slope and its product with 1/2 too."""
+    best = math.log((1 - smoothing) / smoothing) if smoothing else 5.0
+    deltas = np.concatenate([best + np.array([1e-2, 1e-4, -1e-5, 1e-6, -3e-7, 0.1]), np.array([0.0, 1.0, -2.0, 30.0, -30.0, 300.0, -300.0])])
+    pairs = len(deltas)
+    ref = np.zeros((pairs, 2), np.float32)
+    ref[:, 0] = -math.log(2.0) - deltas / beta
+    u = beta * ((-3 * math.log(2.0) - ref[:, 0].astype(np.float64)) + 2 * math.log(2.0))
+    begin = torch.cat([torch.tensor([5 * k, 5 * k + 3], dtype=torch.int32) for k in range(pairs)] + [torch.tensor([5 * pairs], dtype=torch.int32)])
+    x = torch.zeros(5 * pairs, 2, device="cuda")
+    moves = torch.zeros(5 * pairs, dtype=torch.int32, device="cuda")
+    got = learner.preference_loss(x, moves, begin.cuda(), ref_logprob=torch.from_numpy(ref.reshape(-1)).cuda(), beta=beta,
+                                  label_smoothing=smoothing, scale=1.0)
+    margin = got.margin.double().cpu().numpy()
+    assert (np.abs(margin - u) <= U * np.abs(u) + 1e-15).all()
+    with np.errstate(over="ignore"):
+        slope = -beta * ((1 - smoothing) / (1 + np.exp(u)) - smoothing / (1 + np.exp(-u)))
+        loss = ((1 - smoothing) * np.logaddexp(0, -u) + smoothing * np.logaddexp(0, u)).sum()
+    grad = got.grad.double().cpu().numpy().reshape(pairs, 5, 2)
+    sign = np.array([1, 1, 1, -1, -1])[None, :, None] * np.array([0.5, -0.5])[None, None]
+    want = slope[:, None, None] * sign
+    assert (np.abs(grad - want) <= 2.1 * U * np.abs(want) + 2.0 ** -126 + 1e-15).all()
+    assert abs(float(got.loss) - loss) <= 2.1 * U * loss
