@@ -12,6 +12,8 @@
  *     it says so.  A call allocates nothing but in omk_*_create, keeps nothing of its arguments, and holds no work
  *     space of its own: what it needs the caller passes (d_work).  So calls may be captured into graphs, and
  *     graphs replayed side by side, as long as their buffers differ;
+ *   - results and work space lie apart from each other and from all that a call reads; only a gradient by the logits may take
+ *     the logits' place.  Calls whose arguments do not are refused;
  *   - a learner's device need not be the calling thread's: calls put the thread's device back;
  *   - one host thread drives a learner (and its optimizers) at a time.
  *
@@ -72,7 +74,7 @@ typedef struct omk_policy_rows {
 int64_t omk_policy_work(int64_t rows, int32_t actions);
 
 /* Probabilities of the actions, in 32 bits: d_priors[r * prior_stride + j].  What omk_expand_batch takes as
- * h_policy.  d_priors must not overlap the logits. */
+ * h_policy. */
 int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_priors, int64_t prior_stride, void *d_work,
                       int64_t work_bytes);
 
@@ -89,8 +91,7 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
  *   loss  = scale * sum over rows of weight * l
  * and the gradient of the loss by every logit.  (A derivative by lp that passes the 32-bit range is held at its end, so that an
  * illegal action's gradient is 0 beside it too; the loss is infinite there.)  An advantage of 0 gives no loss at whatever ratio, and a row of weight 0
- * adds nothing to loss and gradient, whatever its other columns hold.  Results of a row each (d_logprob, d_kl) must not
- * overlap what is read. */
+ * adds nothing to loss and gradient, whatever its other columns hold. */
 typedef struct omk_policy_samples {
     const int32_t *d_moves;
     const float *d_old_logprob;
@@ -122,7 +123,7 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
  * count nothing) and u_k = beta * ((S_2k - ref_2k) - (S_2k+1 - ref_2k+1)):
  *   loss = scale * sum over pairs of -(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)
  * d_ref_logprob[s] = the line's sum under the reference policy (NULL: 0); a call without d_grad on the reference's logits
- * gives it as d_line_logprob (which must not overlap it).  d_line_begin must not decrease.  (Bounds that do not fit
+ * gives it as d_line_logprob.  d_line_begin must not decrease.  (Bounds that do not fit
  * are taken as the nearest that do: the first and the last inside [0, rows], the others between these two; a line that would end before it begins is
  * empty; which line's gradient a row of two lines gets is open.)  Rows before the first line and behind the last are not
  * read.  0 .. OMK_MAX_PAIRS pairs; with 0 the loss is 0, and every row is a row of no line (zero_rest). */

@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <new>
 #include <utility>
 #include <vector>
@@ -124,6 +125,47 @@ int check_work(const char *who, const void *d_work, int64_t work_bytes, int64_t 
     return OMK_OK;
 }
 
+// Bytes of memory, or of every row of a matrix.
+struct Piece {
+    const void *at;
+    int64_t bytes, stride = 0, rows = 1;
+};
+
+bool across(const Piece &a, const Piece &b) {
+    if (!a.at || !b.at || !a.bytes || !b.bytes) return false;
+    if (a.rows > 1 && b.rows > 1)  // (two matrices: what lies between rows counts)
+        return overlap(a.at, (a.rows - 1) * a.stride + a.bytes, b.at, (b.rows - 1) * b.stride + b.bytes);
+    if (a.rows > 1) return across(b, a);
+    // the first of b's rows that ends behind a's beginning
+    const int64_t from = (int64_t)((uintptr_t)a.at - (uintptr_t)b.at);
+    const int64_t row = from < b.bytes || b.rows < 2 ? 0 : (from - b.bytes) / b.stride + 1;
+    return row < b.rows && overlap(a.at, a.bytes, (const char *)b.at + row * b.stride, b.bytes);
+}
+
+Piece logits_of(const omk_policy_rows *r) {
+    const int width = width_of(r->type);
+    return {r->d_logits, (int64_t)r->actions * width, r->row_stride * width, r->rows};
+}
+Piece legal_of(const omk_policy_rows *r) {
+    return {r->d_legal, (int64_t)((r->actions + 31) / 32) * 4, r->legal_stride * 4, r->legal_stride ? r->rows : 1};
+}
+// A matrix of results beside the logits.
+Piece matrix_of(const omk_policy_rows *r, const void *d, int64_t stride, int width) {
+    return {d, (int64_t)r->actions * width, stride * width, r->rows};
+}
+
+// Results, work space among them, lie apart from each other and from all that is read.  (The first is a matrix, which
+// check_result has held against the logits, the first of what is read.)
+int check_apart(const char *who, std::initializer_list<Piece> results, std::initializer_list<Piece> reads) {
+    for (const Piece *a = results.begin(); a != results.end(); a++) {
+        for (const Piece *b = reads.begin() + (a == results.begin()); b != reads.end(); b++)
+            if (across(*a, *b)) return learn_fail(OMK_ERR_INVALID, "%s: a result lies across what is read", who);
+        for (const Piece *b = a + 1; b != results.end(); b++)
+            if (across(*a, *b)) return learn_fail(OMK_ERR_INVALID, "%s: two results lie across each other", who);
+    }
+    return OMK_OK;
+}
+
 bool aligned4(const char *who, const void *const *p, int n) {
     for (int i = 0; i < n; i++)
         if (!aligned(p[i], 4)) {
@@ -188,7 +230,10 @@ int omk_policy_priors(omk_learner *l, const omk_policy_rows *rows, float *d_prio
     if (int rc = check_rows(who, rows, &r)) return rc;
     if (!r.rows) return OMK_OK;
     if (int rc = check_result(who, "priors", rows, d_priors, prior_stride, 4, false)) return rc;
-    if (int rc = check_work(who, d_work, work_bytes, omk_policy_work(r.rows, r.actions))) return rc;
+    const int64_t work = omk_policy_work(r.rows, r.actions);
+    if (int rc = check_work(who, d_work, work_bytes, work)) return rc;
+    if (int rc = check_apart(who, {matrix_of(rows, d_priors, prior_stride, 4), {d_work, work}}, {logits_of(rows), legal_of(rows)}))
+        return rc;
     OnDevice on(l->device);
     LEARN_TRY(on.status);
     LEARN_TRY(launch_priors(rows->type, r, d_priors, prior_stride, d_work, l->stream));
@@ -205,7 +250,11 @@ int omk_policy_logprobs(omk_learner *l, const omk_policy_rows *rows, const int32
     const void *all[] = {d_moves, d_logprob, d_entropy};
     if (!aligned4(who, all, 3)) return OMK_ERR_INVALID;
     if (!r.rows || (!d_logprob && !d_entropy)) return OMK_OK;
-    if (int rc = check_work(who, d_work, work_bytes, omk_policy_work(r.rows, r.actions))) return rc;
+    const int64_t work = omk_policy_work(r.rows, r.actions), column = r.rows * 4;
+    if (int rc = check_work(who, d_work, work_bytes, work)) return rc;
+    if (int rc = check_apart(who, {{nullptr, 0}, {d_logprob, column}, {d_entropy, column}, {d_work, work}},
+                             {logits_of(rows), legal_of(rows), {d_logprob ? d_moves : nullptr, column}}))
+        return rc;
     OnDevice on(l->device);
     LEARN_TRY(on.status);
     LEARN_TRY(launch_logprobs(rows->type, r, d_moves, d_logprob, d_entropy, d_work, l->stream));
@@ -239,12 +288,14 @@ int omk_policy_loss(omk_learner *l, const omk_policy_rows *rows, const omk_polic
         if (out->d_grad)
             if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true))
                 return rc;
-        const void *results[] = {out->d_logprob, out->d_kl};
-        for (const void *to : results)
-            for (int i = 0; i < 5; i++)  // (the columns that are read come first in `all`)
-                if (to && all[i] && overlap(to, r.rows * 4, all[i], r.rows * 4))
-                    return learn_fail(OMK_ERR_INVALID, "%s: a result lies across what is read", who);
-        if (int rc = check_work(who, d_work, work_bytes, omk_policy_loss_work(r.rows, r.actions))) return rc;
+        const int64_t work = omk_policy_loss_work(r.rows, r.actions), column = r.rows * 4;
+        if (int rc = check_work(who, d_work, work_bytes, work)) return rc;
+        if (int rc = check_apart(who,
+                                 {matrix_of(rows, out->d_grad, out->grad_stride, width_of(rows->type)), {out->d_loss, 4},
+                                  {out->d_logprob, column}, {out->d_kl, column}, {d_work, work}},
+                                 {logits_of(rows), legal_of(rows), {samples->d_moves, column}, {samples->d_old_logprob, column},
+                                  {samples->d_advantage, column}, {samples->d_ref_logprob, column}, {samples->d_weight, column}}))
+            return rc;
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);
@@ -303,15 +354,15 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
         if (int rc = check_result(who, "gradient", rows, out->d_grad, out->grad_stride, width_of(rows->type), true)) return rc;
     if (pairs) {
         if (!d_line_begin || (r.rows && !d_moves)) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
-        const struct {
-            const void *to;
-            int64_t bytes;
-        } results[] = {{out->d_margin, pairs * 4}, {out->d_line_logprob, pairs * 8}};
-        for (const auto &x : results)
-            if (x.to && ((d_ref_logprob && overlap(x.to, x.bytes, d_ref_logprob, pairs * 8)) ||
-                         overlap(x.to, x.bytes, d_line_begin, pairs * 8 + 4)))
-                return learn_fail(OMK_ERR_INVALID, "%s: a result lies across what is read", who);
-        if (int rc = check_work(who, d_work, work_bytes, omk_preference_loss_work(r.rows, r.actions, pairs))) return rc;
+        const int64_t work = omk_preference_loss_work(r.rows, r.actions, pairs);
+        if (int rc = check_work(who, d_work, work_bytes, work)) return rc;
+        const bool some = r.rows > 0;
+        if (int rc = check_apart(who,
+                                 {matrix_of(rows, some ? out->d_grad : nullptr, out->grad_stride, width_of(rows->type)),
+                                  {out->d_loss, 4}, {out->d_margin, pairs * 4}, {out->d_line_logprob, pairs * 8}, {d_work, work}},
+                                 {some ? logits_of(rows) : Piece{nullptr, 0}, some ? legal_of(rows) : Piece{nullptr, 0},
+                                  {d_moves, r.rows * 4}, {d_line_begin, pairs * 8 + 4}, {d_ref_logprob, pairs * 8}}))
+            return rc;
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);
