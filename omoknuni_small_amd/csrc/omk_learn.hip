@@ -560,6 +560,7 @@ int omk_adamw_step(omk_adamw *o, const void *const *h_grads, double lr, const fl
 int omk_adamw_set_steps(omk_adamw *o, int64_t steps) {
     const char *who = "omk_adamw_set_steps";
     if (!o) return learn_fail(OMK_ERR_INVALID, "%s: null argument", who);
+    if (o->l->released) return learn_fail(OMK_ERR_STATE, "%s: the learner has been destroyed", who);
     if (steps < 0 || steps > INT32_MAX) return learn_fail(OMK_ERR_INVALID, "%s: %lld steps", who, (long long)steps);
     OnDevice on(o->l->device);
     LEARN_TRY(on.status);
@@ -570,6 +571,7 @@ int omk_adamw_set_steps(omk_adamw *o, int64_t steps) {
 
 int omk_adamw_get_steps(omk_adamw *o, int64_t *h_steps) {
     if (!o || !h_steps) return learn_fail(OMK_ERR_INVALID, "omk_adamw_get_steps: null argument");
+    if (o->l->released) return learn_fail(OMK_ERR_STATE, "omk_adamw_get_steps: the learner has been destroyed");
     OnDevice on(o->l->device);
     LEARN_TRY(on.status);
     AdamCount c;
