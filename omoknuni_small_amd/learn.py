@@ -465,7 +465,8 @@ class AdamW:
         return n.value
 
     def load_state(self, steps, m, v, m_scale=None, v_scale=None):
-        """Takes over moments laid out as state() gives them, and the count of the steps that made them."""
+        """Takes over moments laid out as state() gives them, and the count of the steps that made them; all of it, or where
+        something is refused nothing."""
         given = dict(m=m, v=v)
         if self.states == "f8":
             given.update(m_scale=m_scale, v_scale=v_scale)
@@ -473,7 +474,8 @@ class AdamW:
             x = given[name]
             if x is None or x.dtype != mine.dtype or x.shape != mine.shape:
                 raise ValueError("%s: %s %s is wanted" % (name, mine.dtype, tuple(mine.shape)))
+        self.learner._on_stream()
+        # (held to what 64 bits pass on: ctypes would cut a larger number)
+        _check(self._lib.omk_adamw_set_steps(self._h, max(-1, min(int(steps), 1 << 31))))
         for name, mine in self.state().items():
             mine.copy_(given[name])
-        self.learner._on_stream()
-        _check(self._lib.omk_adamw_set_steps(self._h, int(steps)))

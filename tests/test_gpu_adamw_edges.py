@@ -30,3 +30,20 @@ def test_an_optimizer_outlives_its_learner(learner):
     assert lib.omk_adamw_get_steps(opt._h, C.byref(n)) == STATE
     assert lib.omk_adamw_step(opt._h, (C.c_void_p * 1)(p.data_ptr()), 0.1, None, None) == STATE
     opt.close()
+
+
+@pytest.mark.parametrize("states", ["f32", "f8"])
+def test_a_state_is_taken_over_whole_or_not_at_all(learner, states):
+    import omoknuni_small_amd as omk
+    p = torch.ones(300, device="cuda")
+    opt = omk.AdamW(learner, [p], states=states)
+    opt.step([p.clone()], lr=0.1)
+    before = {name: x.clone().view(torch.uint8) for name, x in opt.state().items()}
+    other = {name: torch.zeros_like(x) for name, x in opt.state().items()}
+    for steps in (-1, 1 << 31, (1 << 64) + 5):
+        with pytest.raises(omk.OmkError, match="steps"):
+            opt.load_state(steps=steps, **other)
+    assert opt.steps() == 1
+    assert all(torch.equal(before[name], x.view(torch.uint8)) for name, x in opt.state().items())
+    opt.load_state(steps=7, **other)
+    assert opt.steps() == 7 and all((x.view(torch.uint8) == 0).all() for x in opt.state().values())
