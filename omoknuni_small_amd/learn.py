@@ -161,6 +161,7 @@ class Learner:
         self._types = _types()
         self._empty, self._f32, self._i32 = torch.empty, torch.float32, torch.int32
         self._place = torch.device("cuda", self.device)
+        self._written = torch.autograd.graph.increment_version  # told of tensors that are written in place
         # (the address alone: the stream object of torch.cuda.current_stream costs a microsecond)
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -250,7 +251,8 @@ class Learner:
         """Probabilities of the actions, float32 [rows, actions]: 0 where an action is not legal, and in a row that has
         no legal action."""
         r, rows, actions = self._rows(logits, legal)
-        if out is None:
+        given = out is not None
+        if not given:
             out, stride = self._empty((rows, actions), dtype=self._f32, device=self._place), actions
         else:
             self._same_place("out", out, self._f32)
@@ -261,6 +263,8 @@ class Learner:
         self._on_stream()
         _check(self._lib.omk_policy_priors(self._h, C.byref(r), out.data_ptr(), stride,
                                            None if work is None else work.data_ptr(), need))
+        if given:
+            self._written(out)
         return out
 
     def logprobs(self, logits, moves=None, legal=None, entropy=False):
@@ -301,6 +305,8 @@ class Learner:
         self._on_stream()
         _check(self._lib.omk_policy_loss(self._h, C.byref(r), C.byref(samples), C.byref(params), C.byref(out),
                                          at + 4 * behind, need))
+        if g is grad and g is not None:
+            self._written(g)
         view = small.as_strided
         return PolicyLoss(view((), (), 2 * rows), g, view((rows,), (1,), 0), view((rows,), (1,), rows))
 
@@ -332,6 +338,8 @@ class Learner:
         self._on_stream()
         _check(self._lib.omk_preference_loss(self._h, C.byref(r), d_moves, d_begin, pairs, d_ref, C.byref(params),
                                              C.byref(out), at + 4 * behind, need))
+        if g is grad and g is not None:
+            self._written(g)
         view = small.as_strided
         return PreferenceLoss(view((), (), 3 * pairs), g, view((pairs,), (1,), 0), view((lines,), (1,), pairs))
 
@@ -401,6 +409,9 @@ class AdamW:
                          _NONE if copy_type is None else kinds[copy_type], _F32 if states == "f32" else _F8,
                          float(betas[0]), float(betas[1]), float(eps), int(seed) & 0xFFFFFFFF)
         self._sizes = [p.numel() for p in self.params]
+        # what holds the version counters of all that a step writes: views share their base's
+        written = [x if x._base is None else x._base for x in self.params + (self.copies or [])]
+        self._written = list({id(x): x for x in written}.values())
         learner._on_stream()
         _check(self._lib.omk_adamw_create(learner._h, C.byref(desc), C.byref(self._h)))
 
@@ -448,6 +459,13 @@ class AdamW:
         learner._on_stream()
         addresses = array.array("Q", at)
         _check(self._lib.omk_adamw_step(self._h, addresses.buffer_info()[0], number, d_lr, d_scale))
+        # a backward pass that has saved a weight from before this step is refused by torch, as after its own optimizers' steps
+        if 0 not in at:
+            learner._written(self._written)
+        else:
+            learner._written([x for x, g in zip(self.params, at) if g])
+            if self.copies:
+                learner._written([x for x, g in zip(self.copies, at) if g])
 
     def state(self):
         """The moments, as they are held: dict(m, v) and with 8-bit states (float8_e4m3fn, v's square root) m_scale and
