@@ -80,6 +80,7 @@ _ARGTYPES = {
 _ready = None
 _DTYPE = operator.attrgetter("dtype")
 _F32, _BF16, _F16, _F8, _NONE = 0, 1, 2, 3, -1
+_SMALL = 32768  # 128 KB.  (An allocation for the loss alone takes 1.6 us of a call of 17, until the kernels take longer than the call.)
 
 
 def _library():
@@ -236,6 +237,11 @@ class Learner:
             raise ValueError("grad of shape %s, logits of %s" % (tuple(grad.shape), tuple(logits.shape)))
         return grad
 
+    def _loss(self, small, at):
+        """Where a loss is written: at `at` of the memory of a call's other small results, or where that is large in memory of
+        its own, so that a program that keeps its losses keeps little else with them."""
+        return small.as_strided((), (), at) if small.numel() <= _SMALL else self._empty((), dtype=self._f32, device=self._place)
+
     def _work(self, rows, actions):
         """Work space of the calls that need some for wide rows only."""
         need = self._lib.omk_policy_work(rows, actions)
@@ -300,7 +306,8 @@ class Learner:
         behind = (2 * rows + 4) // 4 * 4
         small = old_logprob.new_empty(behind + (need + 3) // 4)
         at = small.data_ptr()
-        out = _PolicyOut(at + 8 * rows, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
+        loss = self._loss(small, 2 * rows)
+        out = _PolicyOut(loss.data_ptr(), None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                          at + 4 * rows)
         self._on_stream()
         _check(self._lib.omk_policy_loss(self._h, C.byref(r), C.byref(samples), C.byref(params), C.byref(out),
@@ -308,7 +315,7 @@ class Learner:
         if g is grad and g is not None:
             self._written(g)
         view = small.as_strided
-        return PolicyLoss(view((), (), 2 * rows), g, view((rows,), (1,), 0), view((rows,), (1,), rows))
+        return PolicyLoss(loss, g, view((rows,), (1,), 0), view((rows,), (1,), rows))
 
     def preference_loss(self, logits, moves, line_begin, ref_logprob=None, legal=None, beta=0.1, label_smoothing=0.0,
                         scale=None, grad=True):
@@ -333,7 +340,8 @@ class Learner:
         behind = (3 * pairs + 4) // 4 * 4
         small = self._empty(behind + (need + 3) // 4, dtype=f32, device=self._place)
         at = small.data_ptr()
-        out = _PreferenceOut(at + 12 * pairs, None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
+        loss = self._loss(small, 3 * pairs)
+        out = _PreferenceOut(loss.data_ptr(), None if g is None else g.data_ptr(), 0 if g is None else g.stride(0), at,
                              at + 4 * pairs, grad is True)
         self._on_stream()
         _check(self._lib.omk_preference_loss(self._h, C.byref(r), d_moves, d_begin, pairs, d_ref, C.byref(params),
@@ -341,7 +349,7 @@ class Learner:
         if g is grad and g is not None:
             self._written(g)
         view = small.as_strided
-        return PreferenceLoss(view((), (), 3 * pairs), g, view((pairs,), (1,), 0), view((lines,), (1,), pairs))
+        return PreferenceLoss(loss, g, view((pairs,), (1,), 0), view((lines,), (1,), pairs))
 
 
 class AdamW:

@@ -284,3 +284,14 @@ def test_slopes_of_pairs_next_to_their_least_loss(learner, beta, smoothing):
     want = slope[:, None, None] * sign
     assert (np.abs(grad - want) <= 2.1 * U * np.abs(want) + 2.0 ** -126 + 1e-15).all()
     assert abs(float(got.loss) - loss) <= 2.1 * U * loss
+
+
+@pytest.mark.parametrize("rows,actions", [(3, 7), (4096, 7), (10000, 7), (100000, 7), (2000, 70001)])
+def test_a_kept_loss_keeps_little(learner, rows, actions):
+    """The memory that a loss holds on to, once all else of its call is gone."""
+    x = torch.zeros(rows, actions, device="cuda", dtype=torch.bfloat16)
+    moves, f = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda")
+    got = learner.policy_loss(x, moves, f - math.log(actions), f + 1, grad=False)
+    assert got.loss.untyped_storage().nbytes() <= 131072 and abs(float(got.loss) + 1) < 1e-5
+    got = learner.preference_loss(x, moves, torch.tensor([0, rows // 2, rows], dtype=torch.int32, device="cuda"), scale=0.0, grad=False)
+    assert got.loss.untyped_storage().nbytes() <= 131072 and float(got.loss) == 0
