@@ -111,12 +111,13 @@ PreferenceLoss = collections.namedtuple("PreferenceLoss", "loss grad margin logp
 
 
 def pack_legal(mask):
-    """A [.., actions] tensor of truth values as [.., words] int32 masks: bit i of word i // 32."""
+    """A [.., actions] tensor of truth values (or numbers, 0 where an action is not legal) as [.., words] int32 masks: bit i of
+    word i // 32."""
     torch = _torch()
     actions = mask.shape[-1]
     words = (actions + 31) // 32
     bits = torch.zeros(mask.shape[:-1] + (words * 32,), dtype=torch.int64, device=mask.device)
-    bits[..., :actions] = mask
+    bits[..., :actions] = mask != 0
     packed = (bits.unflatten(-1, (words, 32)) << torch.arange(32, device=mask.device)).sum(-1)
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32)
 

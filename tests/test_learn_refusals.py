@@ -1,6 +1,8 @@
 """Refusals of include/omk_learn.h beyond those of test_learn_host.py, without a GPU: each before anything is enqueued."""
 import ctypes as C
 
+import pytest
+
 from omoknuni_small_amd import learn
 from tests.test_learn_host import INVALID, address, handle, message, policy, preference, rows  # noqa: F401  (handle: a fixture)
 
@@ -65,3 +67,12 @@ def test_what_lies_between_rows_is_free(handle):  # noqa: F811
         assert across(policy(handle, out=dict(d_loss=begin + 448), r=r)) and across(policy(handle, out=dict(d_loss=begin), r=r))
         got = policy(handle, out=dict(d_loss=begin + 452), r=r)
         assert got not in (0, INVALID) and "across" not in message()
+
+
+def test_masks_of_numbers():
+    """Masks that are no truth values: what is not 0 is legal, whatever its size."""
+    torch = pytest.importorskip("torch")
+    mask = torch.rand(5, 70, generator=torch.Generator().manual_seed(1)) < 0.5
+    want = learn.pack_legal(mask)
+    for values in (mask.to(torch.uint8) * 255, mask.int() * 2, mask.long() * -7, mask.float() * 0.25, mask.half() * 3.5):
+        assert torch.equal(learn.pack_legal(values), want), values.dtype
