@@ -187,6 +187,12 @@ __device__ __forceinline__ double in_range(double slope) {
     return slope > most ? most : slope < -most ? -most : slope;
 }
 
+// 1 / x for 1 <= x < 2^30: a 32-bit one, a step off, and Newton's step in 64 bits (good to 2^-44).
+__device__ __forceinline__ double reciprocal(double x) {
+    const double r = (double)__builtin_amdgcn_rcpf((float)x);
+    return r * __builtin_fma(-x, r, 2.0);
+}
+
 struct PolicyOp {
     static constexpr bool kCentred = false, kElements = true, kMoves = true, kLoss = true;
     template <typename T>
@@ -213,7 +219,9 @@ struct PolicyOp {
         if (m.chosen != -INFINITY) {
             const double exact = (double)m.chosen - (double)s.top - log(s.sum);
             lp = (float)exact;
-            if (p.grad) others = 1.0 - exp(exact);
+            // (a move with more than half of the probability has the largest logit, whose term is 1 exactly: nothing is lost of S - 1;
+            // and beside a smaller term's S - e its rounding is nothing.  An exponential in 64 bits took 0.8 us of 69 on 131072 rows of 362.)
+            if (p.grad) others = (s.sum - (double)exp_of<true>(at_least(m.chosen - s.top, -200.0f))) * reciprocal(s.sum);
             const float a = p.advantage[row];
             const double shift = exact - (double)p.old_logprob[row];
             if (a > 0.0f ? shift > p.log_high : a < 0.0f && shift < p.log_low) {
