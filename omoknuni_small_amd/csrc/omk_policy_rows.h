@@ -833,7 +833,7 @@ static Launched run_stream(const Rows &r, const OP &op, hipStream_t stream) {
 }
 
 // Wavefronts that fill the card: eight on each of 256 compute units.  (Rows of 362 bf16 with their gradient: 4096 of them
-// take 6.7 us with 64 lanes each and 7.2 us with 16, 8192 10.7 and 8.4 us, 16384 17.1 and 13.2 us; 131072 83 and 59 us.)
+// take 8.0 us with 64 lanes each and 8.9 us with 16, 8192 12.7 and 9.7 us, 16384 21.3 and 15.0 us, 131072 130 and 71 us.)
 constexpr int64_t kFullOfRows = 256 * 8;
 
 template <bool ONCE, typename T, typename OP>
@@ -841,7 +841,7 @@ static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_
     const int64_t n = vectors_of<T>(r);
     // Few rows are done soonest with a lane for every vector; where the card is full of wavefronts all the same, many
     // rows to a wavefront: four vectors a lane and 16 lanes at least (with 8 a store's pieces are shorter than a cache
-    // line: 131072 rows of 225 floats took 74 us, with 16 lanes 62).
+    // line: 131072 rows of 225 floats took a fifth longer than with 16).
     if (n <= 256) {
         const auto full = [&](int team) { return r.rows >= kFullOfRows * (64 / team); };
         if (n <= 32 && full(16)) return run_narrow<ONCE, T, 16, 2>(r, op, stream);
@@ -861,9 +861,9 @@ static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_
         if constexpr (sizeof(T) == 4)
             if (n <= 16384) return run_rows<ONCE, T, 1024, 16>(r, op, stream);
     } else if (n <= 16384) {
-        // (2 waves of 256 compute units' blocks: 512 rows of 32768 bf16 take 14.2 us with blocks of 1024 and 15.8 us with
-        // blocks of 256, 64 rows 7.5 and 11.2 us, 1024 rows 22.1 and 18.2 us)
-        return r.rows <= 512 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
+        // (up to a row for every compute unit: 64 rows of 32768 bf16 take 6.9 us with blocks of 1024 and 9.0 us with blocks of 256,
+        // 256 rows 7.6 and 9.5 us, 384 rows 13.3 and 12.8 us, 512 rows 14.0 and 13.2 us, 1024 rows 21.1 and 18.6 us)
+        return r.rows <= 256 ? run_stream<ONCE, T, 1024>(r, op, stream) : run_stream<ONCE, T, 256>(r, op, stream);
     }
     OP o = op;
     if constexpr (OP::kLoss)
@@ -874,8 +874,8 @@ static Launched run_class(const Rows &r, const OP &op, const Wide &w, hipStream_
 }
 
 // Logits that the second-level caches (4 MB on each of the card's eight dies) cannot hold together are not kept in them:
-// 8192 rows of 32768 bf16 take 204 us with nontemporal accesses and 229 us without, 131072 of 362 (95 MB) 60 and 71 us,
-// 32768 of 362 floats (47 MB) 26.8 and 26.5 us.
+// 8192 rows of 32768 bf16 take 221 us with nontemporal accesses and 233 us without, 131072 of 362 (95 MB) 70 and 76 us,
+// 32768 of 362 floats (47 MB) 29.4 and 28.1 us.
 static inline bool met_once(const Rows &r, int width) { return r.rows * (int64_t)r.actions * width > (int64_t)32 << 20; }
 
 template <typename T, typename OP>
