@@ -24,7 +24,7 @@
  * A row without a legal action, or with -inf in all of them, has no policy: probabilities and entropy are 0.  A row
  * that has no policy, or whose move lies outside [0, actions) (a padded position: -1) or is not legal (or has the
  * logit -inf), is LEFT OUT of a loss: its loss, log-probability and gradient are 0.  A NaN or +inf among the legal
- * logits makes its row's results NaN.
+ * logits makes its row's results NaN, in the columns of illegal actions too.
  */
 #ifndef OMK_LEARN_H
 #define OMK_LEARN_H
@@ -153,7 +153,9 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
  * of the tensor (its last block may be shorter); the largest magnitude of a block becomes 448, and the others are
  * rounded up or down at random with the probability of their place between two codes (random numbers from seed, t and
  * the element's place, so a run repeats): to the nearest, a second moment that changes by a thousandth a step would
- * never leave its code.  A sqrt(v) that is not 0 keeps the smallest code at least. */
+ * never leave its code.  A sqrt(v) that is not 0 keeps the smallest code at least.
+ * An infinite gradient or a NaN stays in the moments, as in the formula, and with states in 8 bits in those of all 256 elements
+ * that share its scale: look at gradients before the step (a step is not left out on the device). */
 typedef struct omk_adamw_tensor {
     int64_t n;
     void *d_param;

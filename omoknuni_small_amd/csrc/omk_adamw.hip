@@ -7,7 +7,7 @@ namespace omk {
 
 constexpr int kAdamBlock = 256;
 
-// Mixes the bits of a number: xorshifts and products with odd constants, every input bit reaching every output bit.
+// Mixes the bits of a number: the published 32-bit integer hash "lowbias32" (C. Wellons, 2018), its shifts and constants.
 __device__ __forceinline__ uint32_t mix(uint32_t h) {
     h ^= h >> 16;
     h *= 0x7FEB352Du;

@@ -453,8 +453,8 @@ __global__ __launch_bounds__(256) void k_narrow(Rows r, OP op) {
 // Wider rows: a block of TEAM threads holds a row, K vectors a thread.
 //
 // What bounds it is memory's rate, if enough loads are on their way: a block that waits for its row's reductions loads
-// nothing, so a compute unit needs two of the largest blocks (at most 64 registers a thread).  8192 rows of 32768 bf16
-// with their gradient take 204 to 214 us with two (5.0 to 5.3 TB/s), 313 us with one (229 without nontemporal accesses).
+// nothing, so a compute unit needs two of the largest blocks (at most 64 registers a thread; with one at a time these rows took
+// half as much again).  8192 rows of 32768 bf16 with their gradient take 206 to 212 us one call behind another (5.1 to 5.2 TB/s).
 template <bool ONCE, typename T, int TEAM, int K, typename OP>
 __global__ __launch_bounds__(TEAM, TEAM == 1024 && K <= 4 ? 8 : 1) void k_rows(Rows r, OP op) {
     constexpr int V = Pack<T>::V, WAVES = TEAM / 64;
@@ -723,7 +723,7 @@ __device__ __forceinline__ double block_sum(const F *values, int64_t n) {
 }
 
 // The gradient's slope is known only when the last row of a pair has been read, so that logits are read twice: 9728 rows of
-// 32768 bf16 (638 MB) in 321 us, of which the first reading takes 109 us (5.8 TB/s) and this, which reads again and writes, 211 us
+// 32768 bf16 (638 MB) in 335 us, of which the first reading takes 122 us (5.2 TB/s) and this, which reads again and writes, 211 us
 // (6.0 TB/s).
 // Two and eight vectors a lane took a fifth longer than four.
 // A wavefront takes kGradientVectors * 64 vectors of a row.  The first block also adds the pairs' losses up.

@@ -464,7 +464,8 @@ class Batch:
 
     def expand_logits(self, move_begin, moves, logits, learner, widening=None):
         """expand_ex() with the priors that the network's logits give: logits [n, action_space] are on the GPU (a row a
-        traversal, as learner.priors takes them), and a leaf's priors are their softmax over the moves it offers.
+        traversal, as learner.priors takes them), and a leaf's priors are their softmax over the moves it offers (a move outside the
+        action space has no logit, and the prior that expand_ex() gives it).
         Waits for the logits."""
         from .learn import legal_of_moves
         n = len(move_begin) - 1

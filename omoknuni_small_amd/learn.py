@@ -7,7 +7,8 @@ there when a call is made, and waits for nothing.  Every call goes through libom
 Import torch before anything here or in forest.py loads that library: the two then share one HIP runtime (a torch that brings its
 own and comes second finds no GPU; Learner says so).
 
-A gradient by the logits is handed on to the network that made them: `logits.backward(got.grad)`.
+A gradient by the logits is handed on to the network that made them: `logits.backward(got.grad)`.  That is the only way back:
+results carry no history of their own (neither requires_grad nor forward-mode tangents), whatever the logits carry.
 """
 import array
 import collections
@@ -356,7 +357,8 @@ class Learner:
 class AdamW:
     """AdamW over many tensors at once (omk_adamw), stepped in place by one launch for every 256 of them.
 
-    params: contiguous tensors of one type on the learner's device; they stay where they are while the optimizer lives.
+    params: contiguous tensors of one type on the learner's device; they stay where they are while the optimizer lives.  (Also of
+    four dimensions: weights and gradients in a channels-last layout are refused.)
     copies: 16-bit tensors that take the rounded parameters with every step (32-bit parameters only).  grad_type: the
     gradients' type (None: the parameters').  states: "f32", or "f8" for moments in 8 bits with a scale for every 256
     elements.  weight_decay, lr_scale: one value, or one for every tensor.
@@ -436,7 +438,8 @@ class AdamW:
             pass
 
     def step(self, grads, lr, grad_scale=None):
-        """One step.  grads: a contiguous tensor of grad_type for every parameter, or None where one has none (it is left
+        """One step.  An infinite or NaN gradient stays in the moments (with 8-bit ones in its block of 256): nothing is skipped.
+        grads: a contiguous tensor of grad_type for every parameter, or None where one has none (it is left
         as it is).  lr: a number, or a float32 tensor of one value on the device.  grad_scale: a float32 tensor of one
         value that gradients are multiplied by (a clipping factor, one over a loss scale)."""
         if len(grads) != len(self.params):
