@@ -363,6 +363,10 @@ int omk_preference_loss(omk_learner *l, const omk_policy_rows *rows, const int32
                                  {some ? logits_of(rows) : Piece{nullptr, 0}, some ? legal_of(rows) : Piece{nullptr, 0},
                                   {d_moves, r.rows * 4}, {d_line_begin, pairs * 8 + 4}, {d_ref_logprob, pairs * 8}}))
             return rc;
+    } else if (r.rows) {
+        if (int rc = check_apart(who, {matrix_of(rows, out->d_grad, out->grad_stride, width_of(rows->type)), {out->d_loss, 4}},
+                                 {logits_of(rows)}))
+            return rc;
     }
     OnDevice on(l->device);
     LEARN_TRY(on.status);

@@ -76,3 +76,8 @@ def test_masks_of_numbers():
     want = learn.pack_legal(mask)
     for values in (mask.to(torch.uint8) * 255, mask.int() * 2, mask.long() * -7, mask.float() * 0.25, mask.half() * 3.5):
         assert torch.equal(learn.pack_legal(values), want), values.dtype
+
+
+def test_results_lie_apart_without_pairs(handle):  # noqa: F811
+    for at in (address(3), address(3) + LOGITS - 4, address(0), address(0) + LOGITS - 4):
+        assert across(preference(handle, out=dict(d_loss=at, zero_rest=1), pairs=0)), hex(at)
